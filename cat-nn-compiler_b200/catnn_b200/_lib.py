@@ -69,6 +69,17 @@ SIGNATURES = {
     "catnn_swiglu_bwd": [VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I32],
     "catnn_moe_fwd": [VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I32],
     "catnn_moe_bwd": [VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I32],
+    "catnn_qk_norm_rope_fwd": [VP, VP, I64, VP, I64, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, F64, F32, I32],
+    "catnn_qk_norm_rope_bwd_workspace": [VP, I64, I64, I64, I64, I64, C.POINTER(C.c_size_t)],
+    "catnn_qk_norm_rope_bwd": [VP, VP, I64, VP, I64, VP, VP, VP, VP, I64, VP, I64, VP, VP, VP, VP, I64, I64, I64, I64,
+                               I64, F64, F32, I32, VP, C.c_size_t],
+    "catnn_kv_append": [VP, VP, I64, VP, I64, VP, I64, VP, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I64,
+                        I64, I64, F64, F32, I32, I32],
+    "catnn_paged_attention_workspace": [VP, I64, I64, I64, I64, C.POINTER(C.c_size_t)],
+    "catnn_paged_attention_fwd": [VP, VP, I64, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I64, I64, I64, I32, VP,
+                                  C.c_size_t, I32],
+    "catnn_moe_few_workspace": [VP, I64, I64, I64, I64, I64, I32, C.POINTER(C.c_size_t)],
+    "catnn_moe_few_fwd": [VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I32, VP, C.c_size_t],
     "catnn_sgd": [VP, VP, VP, I64, F32, VP],
     "catnn_adam": [VP, VP, VP, VP, VP, I64, U64, F32, F32, F32, F32, I32, VP],
     "catnn_mlp_step": [VP, VP, VP, VP, VP, VP, VP, VP, I32, I64, I64, I64, I64, VP, VP, VP, VP, VP],

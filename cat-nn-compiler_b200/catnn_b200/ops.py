@@ -26,11 +26,24 @@ class Context:
         h = C.c_void_p()
         _lib.call("catnn_ctx_create", int(device), C.byref(h))
         self.handle = h
+        self._workspace = {}
 
     def bind(self):
         s = torch.cuda.current_stream(self.device).cuda_stream
         _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
         return self.handle
+
+    def workspace(self, name, *sizes):
+        """A workspace of the bytes that `name`'s _workspace function asks
+        for, from torch's allocator (so it belongs to the current stream, or
+        to the graph being captured), or None where it asks for none. The
+        sizes asked for are kept, not the memory."""
+        n = self._workspace.get((name, sizes))
+        if n is None:
+            v = C.c_size_t()
+            _lib.call(name, self.handle, *sizes, C.byref(v))
+            n = self._workspace[(name, sizes)] = int(v.value)
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
 
     def launch_count(self):
         v = C.c_uint64()
@@ -513,6 +526,206 @@ def moe_backward(x, gate, w1s, w3s, w2s, dy, top_k):
     _lib.call("catnn_moe_bwd", _h(x), _p(x), _p(gate), _p(w1s), _p(w3s), _p(w2s), _p(dy), *[_p(o) for o in outs], t, h, mid,
               e, top_k, _dt(x))
     return tuple(outs)
+
+
+# ------------------------------------------------------------------ decoding
+def _on(t, *others):
+    """All of one call's tensors lie on one CUDA device."""
+    if not t.is_cuda:
+        raise InvalidArgument("catnn_b200 operators take CUDA tensors")
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise InvalidArgument(f"tensors on {t.device} and {o.device}")
+
+
+def _rows(t, what):
+    """Elements between the tokens of t [..., heads, hd], whose heads must be
+    dense and whose tokens evenly spaced: a tensor of its own, or a column
+    block of the rows that one QKV product writes."""
+    *lead, heads, hd = t.shape
+    st = t.stride()
+    if t.numel() == 0:
+        return heads * hd
+    if (hd > 1 and st[-1] != 1) or (heads > 1 and st[-2] != hd):
+        raise InvalidArgument(f"{what}: a token's heads must be dense")
+    step = None  # stride of the next inner token dimension, times its size
+    for n, s in zip(reversed(lead), reversed(st[:-2])):
+        if n == 1:
+            continue
+        if step is None:
+            token, step = s, s * n
+        elif s != step:
+            raise InvalidArgument(f"{what}: tokens must be evenly spaced")
+        else:
+            step = s * n
+    return heads * hd if step is None else token
+
+
+def _i32(t, what):
+    if t.dtype != torch.int32:
+        raise DTypeMismatch(f"{what} must be int32")
+    if not t.is_contiguous():
+        raise InvalidArgument(f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _weight(w, hd, what):
+    if w.dtype != torch.float32:
+        raise DTypeMismatch(f"{what} must be float32")
+    if w.shape != (hd,) or (hd > 1 and w.stride(0) != 1):
+        raise ShapeMismatch(f"{what} must be a dense [{hd}] vector")
+    return w.data_ptr()
+
+
+def _qk(q, k, wq, wk, positions, what):
+    _same(q, k)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ShapeMismatch(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if positions is not None and positions.shape != q.shape[:2]:
+        raise ShapeMismatch(f"{what}: positions {tuple(positions.shape)}")
+    _on(q, k, wq, wk, positions)
+    return None if positions is None else _i32(positions, "positions")
+
+
+def qk_norm_rope(q, k, wq, wk, theta, eps=1e-5, positions=None):
+    """RMS norm of every head of q [B,S,H,hd] and k [B,S,Hkv,hd] with the
+    weights wq, wk [hd] (fp32), then the rotation of its pairs to its position,
+    in one pass -> (q', k'), dense. positions int32 [B,S]; None: 0..S-1. q and k
+    may be column blocks of packed QKV rows."""
+    pos = _qk(q, k, wq, wk, positions, "qk_norm_rope")
+    b, s, h, hd = q.shape
+    hkv = k.shape[2]
+    qo = torch.empty((b, s, h, hd), dtype=q.dtype, device=q.device)
+    ko = torch.empty((b, s, hkv, hd), dtype=q.dtype, device=q.device)
+    _lib.call("catnn_qk_norm_rope_fwd", _h(q), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
+              _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, qo.data_ptr(), ko.data_ptr(), b, s, h, hkv, hd, theta, eps,
+              _dt(q))
+    return qo, ko
+
+
+def qk_norm_rope_backward(q, k, wq, wk, dq_out, dk_out, theta, eps=1e-5, positions=None):
+    """Adjoint of qk_norm_rope from its inputs and the gradients of its
+    results -> (dq, dk, dwq, dwk); dwq and dwk are summed in a fixed order."""
+    _same(q, dq_out, dk_out)
+    if dq_out.shape != q.shape or dk_out.shape != k.shape:
+        raise ShapeMismatch(f"qk_norm_rope backward: dq_out {tuple(dq_out.shape)}, dk_out {tuple(dk_out.shape)}")
+    pos = _qk(q, k, wq, wk, positions, "qk_norm_rope backward")
+    _on(q, dq_out, dk_out)
+    b, s, h, hd = q.shape
+    hkv = k.shape[2]
+    ctx = context(q.device)
+    ws = ctx.workspace("catnn_qk_norm_rope_bwd_workspace", b, s, h, hkv, hd)
+    dq = torch.empty((b, s, h, hd), dtype=q.dtype, device=q.device)
+    dk = torch.empty((b, s, hkv, hd), dtype=q.dtype, device=q.device)
+    dw = torch.empty((2, hd), dtype=torch.float32, device=q.device)
+    _lib.call("catnn_qk_norm_rope_bwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
+              _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, dq_out.data_ptr(), _rows(dq_out, "dq_out"),
+              dk_out.data_ptr(), _rows(dk_out, "dk_out"), dq.data_ptr(), dk.data_ptr(), dw.data_ptr(),
+              dw.data_ptr() + 4 * hd, b, s, h, hkv, hd, theta, eps, _dt(q), None if ws is None else ws.data_ptr(),
+              0 if ws is None else ws.numel())
+    return dq, dk, dw[0], dw[1]
+
+
+def _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, like, what):
+    _same(like, k_cache, v_cache)
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != hkv or k_cache.shape[3] != hd:
+        raise ShapeMismatch(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} for {hkv} heads of {hd}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise InvalidArgument(f"{what}: caches must be contiguous")
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0]:
+        raise ShapeMismatch(f"{what}: page table {tuple(page_table.shape)}, lengths {tuple(seq_lens.shape)}")
+    ptrs = _i32(page_table, "page_table"), _i32(seq_lens, "seq_lens")
+    _on(like, k_cache, v_cache, page_table, seq_lens)
+    return ptrs
+
+
+def kv_append(q, k, v, k_cache, v_cache, page_table, seq_lens, theta, cu_tokens=None, wq=None, wk=None, eps=1e-5,
+              check=False):
+    """Appends the keys and values of new tokens to a paged cache, in place,
+    and returns their rotated queries [T,H,hd] (None for q None).
+
+    q [T,H,hd], k and v [T,Hkv,hd] (column blocks of packed QKV rows, or
+    tensors of their own); caches [pages,Hkv,page,hd]; page_table int32
+    [seqs,max_pages]; seq_lens int32 [seqs], with the new tokens; cu_tokens
+    int32 [seqs+1]: where each sequence's new tokens begin among the T rows,
+    None for one new token each. wq, wk (fp32 [hd]): per-head RMS norm before
+    the rotation. Rows of no sequence are not appended (their queries are
+    zero); slots without a page are not written, which check=True
+    (synchronizing) reports as a ShapeMismatch. No two rows may name the same
+    slot."""
+    if k.dim() != 3 or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0]
+                                                                 or q.shape[2] != k.shape[2])):
+        raise ShapeMismatch(f"kv_append: q {None if q is None else tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    t, hkv, hd = k.shape
+    h = 0 if q is None else q.shape[1]
+    seqs = page_table.shape[0]
+    _same(k, v, q)
+    if cu_tokens is not None and cu_tokens.shape != (seqs + 1,):
+        raise ShapeMismatch(f"kv_append: cu_tokens {tuple(cu_tokens.shape)} for {seqs} sequences")
+    if (wq is None) != (wk is None):
+        raise InvalidArgument("kv_append: both norm weights or neither")
+    if cu_tokens is None and t != seqs:
+        raise ShapeMismatch(f"kv_append: {t} rows for {seqs} sequences without cu_tokens")
+    table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, k, "kv_append")
+    _on(k, q, v, cu_tokens, wq, wk)
+    qo = None if q is None else torch.empty((t, h, hd), dtype=q.dtype, device=q.device)
+    _lib.call("catnn_kv_append", _h(k), None if q is None else q.data_ptr(), 0 if q is None else _rows(q, "q"),
+              k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), None if wq is None else _weight(wq, hd, "wq"),
+              None if wk is None else _weight(wk, hd, "wk"), None if q is None else qo.data_ptr(), k_cache.data_ptr(),
+              v_cache.data_ptr(), table, lens, None if cu_tokens is None else _i32(cu_tokens, "cu_tokens"), t, seqs, h, hkv,
+              hd, k_cache.shape[0], k_cache.shape[2], page_table.shape[1], theta, eps, _dt(k), int(check))
+    return qo
+
+
+def paged_attention(q, k_cache, v_cache, page_table, seq_lens, window=None, check=False):
+    """Attention of one new token of each sequence, q [seqs,H,hd], against its
+    cached positions, the last of which is its own (append first)
+    -> (o [seqs,H*hd], lse [seqs,H]). Caches, table and lengths as in
+    kv_append; a sequence of length 0 gets zeros and -inf."""
+    if q.dim() != 3:
+        raise ShapeMismatch(f"paged_attention: q {tuple(q.shape)}")
+    b, h, hd = q.shape
+    hkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    if hkv < 1 or h % hkv or seq_lens.shape[0] != b:
+        raise ShapeMismatch(f"paged_attention: q {tuple(q.shape)} for {hkv} kv heads, {tuple(seq_lens.shape)} sequences")
+    table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, q, "paged_attention")
+    ctx = context(q.device)
+    ws = ctx.workspace("catnn_paged_attention_workspace", b, h, hkv, hd)
+    o = torch.empty((b, h * hd), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, h), dtype=torch.float32, device=q.device)
+    _lib.call("catnn_paged_attention_fwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(),
+              table, lens, o.data_ptr(), lse.data_ptr(), b, h, hkv, hd, k_cache.shape[0], k_cache.shape[2],
+              page_table.shape[1], int(window or 0), _dt(q), None if ws is None else ws.data_ptr(),
+              0 if ws is None else ws.numel(), int(check))
+    return o, lse
+
+
+def moe_few(x, gate, w1s, w3s, w2s, top_k):
+    """moe() for at most 64 rows of x, in two kernels that read each chosen
+    expert's weights once; expert weights stacked [E, ...]."""
+    _same(x, gate, w1s, w3s, w2s)
+    hid = x.shape[-1]
+    t = x.numel() // max(hid, 1)
+    if w1s.dim() != 3:
+        raise ShapeMismatch(f"moe_few: w1s {tuple(w1s.shape)}")
+    e, _, mid = w1s.shape
+    if (w1s.shape != (e, hid, mid) or w3s.shape != w1s.shape or w2s.shape != (e, mid, hid) or gate.shape != (hid, e)):
+        raise ShapeMismatch(f"moe_few: x {tuple(x.shape)}, gate {tuple(gate.shape)}, w1s {tuple(w1s.shape)}, "
+                            f"w3s {tuple(w3s.shape)}, w2s {tuple(w2s.shape)}")
+    if not (x.is_contiguous() and gate.is_contiguous() and w1s.is_contiguous() and w3s.is_contiguous()
+            and w2s.is_contiguous()):
+        raise InvalidArgument("catnn_b200 operators take contiguous tensors")
+    if t > 64 or not 1 <= top_k <= e <= 32:
+        raise ShapeMismatch(f"moe_few: {t} rows (at most 64), top {top_k} of {e} experts (at most 32)")
+    dt = _dt(x)
+    _on(x, gate, w1s, w3s, w2s)
+    ctx = context(x.device)
+    ws = ctx.workspace("catnn_moe_few_workspace", t, hid, mid, e, top_k, dt)
+    y = torch.empty_like(x)
+    _lib.call("catnn_moe_few_fwd", ctx.bind(), x.data_ptr(), gate.data_ptr(), w1s.data_ptr(), w3s.data_ptr(),
+              w2s.data_ptr(), y.data_ptr(), t, hid, mid, e, top_k, dt, None if ws is None else ws.data_ptr(),
+              0 if ws is None else ws.numel())
+    return y
 
 
 # ------------------------------------------------------------------ optimizers

@@ -55,6 +55,11 @@ struct Context {
     void* rope_tab = nullptr;
     i64 rope_s = 0, rope_hd = 0;
     double rope_theta = 0.0;
+    // Turns per position of each rotated pair for (theta, head_dim), host
+    // values that kernels take as an argument (qk_norm.cu).
+    double turns[128] = {0.0};
+    i64 turns_hd = 0;
+    double turns_theta = 0.0;
     // Grow-only arena for composite ops (several temporaries held across
     // the leaf launchers, which use `scratch`).
     void* work = nullptr;

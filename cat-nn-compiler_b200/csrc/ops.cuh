@@ -206,4 +206,29 @@ void swiglu_act(Context* c, const void* a, const void* cc, void* h, i64 rows, i6
 void swiglu_act_bwd(Context* c, const void* a, const void* cc, const void* dh, void* da, void* dc, i64 rows,
                     i64 F, i64 lda, i64 ldd, int dtype, int in_dtype = -1, const int32_t* rows_dev = nullptr);
 
+// ---- per-head query/key norm with the rotation, and the paged cache (qk_norm.cu, paged_attention.cu)
+// Strides are elements between tokens; a token's heads are dense. pos null: token % s.
+void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const float* wq, const float* wk,
+                      const int32_t* pos, void* qo, void* ko, i64 b, i64 s, i64 h, i64 hkv, i64 hd, double theta, float eps,
+                      int dtype);
+size_t qk_norm_rope_bwd_workspace(Context* c, i64 b, i64 s, i64 h, i64 hkv, i64 hd);
+void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const float* wq, const float* wk,
+                      const int32_t* pos, const void* gq, i64 gq_stride, const void* gk, i64 gk_stride, void* dq, void* dk,
+                      float* dwq, float* dwk, i64 b, i64 s, i64 h, i64 hkv, i64 hd, double theta, float eps, int dtype,
+                      float* work);
+// err (optional device int): set to 1 where a position has no page in the table or the pool.
+void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const void* v, i64 v_stride,
+               const float* wq, const float* wk, void* qo, void* kc, void* vc, const int32_t* table, const int32_t* lens,
+               const int32_t* cu, i64 tokens, i64 seqs, i64 h, i64 hkv, i64 hd, i64 pages, i64 page, i64 max_pages,
+               double theta, float eps, int dtype, int* err);
+size_t paged_attention_workspace(Context* c, i64 seqs, i64 h, i64 hkv, i64 hd);
+void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, const void* vc, const int32_t* table,
+                     const int32_t* lens, void* o, float* lse, i64 seqs, i64 h, i64 hkv, i64 hd, i64 pages, i64 page,
+                     i64 max_pages, i64 window, int dtype, void* work, int* err);
+
+// ---- a MoE layer for a few tokens (moe_few.cu)
+size_t moe_few_workspace(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k, int dtype);
+void moe_few(Context* c, const void* x, const void* gate, const void* w1, const void* w3, const void* w2, void* y, i64 T,
+             i64 hidden, i64 mid, i64 E, i64 k, int dtype, void* work);
+
 }  // namespace catnn

@@ -275,6 +275,90 @@ int catnn_moe_bwd(catnn_ctx* ctx, const void* x, const void* gate, const void* w
                   const void* w2s, const void* dy, void* dx, void* dgate, void* dw1s, void* dw3s,
                   void* dw2s, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k, int dtype);
 
+/* ------------------------------------------------------------ decoding
+ * What answers with a decoder that the training steps train: per-head
+ * query/key norms with the rotation, a paged key/value cache, attention of
+ * one new token against it, and the MoE block for a few tokens. No
+ * counterpart in the reference, whose kernels recompute whole sequences;
+ * rotation, norm, router and experts are those of moe.rs:17-223.
+ *
+ * Strides are elements between tokens, so q, k and v may be column blocks of
+ * the rows that one QKV product writes; a token's heads are dense [heads,
+ * hd]. Calls that need device memory take it from the caller (`workspace`,
+ * 256-byte aligned, at least the bytes its _workspace function returns; its
+ * contents do not matter and it is free again once the call's work is done),
+ * so that they allocate nothing, synchronize with nothing unless check != 0,
+ * can be captured, and share nothing with calls on other streams. */
+
+/* q' = R(pos)·rmsnorm(q; wq), k' = R(pos)·rmsnorm(k; wk) for each head of
+ * q [b,s,n_heads,hd] and k [b,s,n_kv,hd] (moe.rs:17 over hd, then moe.rs:47):
+ * wq, wk fp32 [hd]; positions int32 [b,s], or NULL for 0..s-1 in every
+ * sequence; angles pos·theta^(-2i/hd) in f64. hd even, at most 256. q_out
+ * [b,s,n_heads,hd] and k_out [b,s,n_kv,hd] are dense and may be the inputs
+ * themselves where those are dense. */
+int catnn_qk_norm_rope_fwd(catnn_ctx* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                           const float* wq, const float* wk, const int32_t* positions, void* q_out, void* k_out,
+                           int64_t b, int64_t s, int64_t n_heads, int64_t n_kv, int64_t hd, double theta, float eps,
+                           int dtype);
+/* Its adjoint from the same q, k (before the norm) and the gradients dq_out,
+ * dk_out of its results: dq, dk dense in `dtype`; dwq, dwk fp32 [hd], summed
+ * over tokens and heads in a fixed order (the same bits on every call). */
+int catnn_qk_norm_rope_bwd_workspace(catnn_ctx* ctx, int64_t b, int64_t s, int64_t n_heads, int64_t n_kv, int64_t hd,
+                                     size_t* bytes);
+int catnn_qk_norm_rope_bwd(catnn_ctx* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                           const float* wq, const float* wk, const int32_t* positions, const void* dq_out,
+                           int64_t dq_out_stride, const void* dk_out, int64_t dk_out_stride, void* dq, void* dk,
+                           float* dwq, float* dwk, int64_t b, int64_t s, int64_t n_heads, int64_t n_kv, int64_t hd,
+                           double theta, float eps, int dtype, void* workspace, size_t workspace_bytes);
+
+/* Appends the keys and values of `tokens` new tokens to a paged cache and
+ * rotates their queries. k_cache, v_cache [n_pages, n_kv, page_size, hd];
+ * position j of sequence i lies in slot j % page_size of page
+ * page_table[i, j / page_size] (int32 [seqs, max_pages]). seq_lens int32
+ * [seqs]: each sequence's length with its new tokens. cu_tokens int32
+ * [seqs+1]: sequence i's new tokens are rows [cu_tokens[i], cu_tokens[i+1]),
+ * its last ones; NULL: row i is the one new token of sequence i. Keys and
+ * queries are rotated to their positions, after a per-head RMS norm where
+ * wq, wk (fp32 [hd], both or neither) are given; values are copied. q and
+ * q_out [tokens, n_heads, hd] (dense) may both be NULL (then n_heads is 0).
+ * Every other slot of the cache is left as it was. Rows that belong to no
+ * sequence (behind the last one, or of a sequence whose length ends before
+ * position 0) are not appended and their q_out is zero. A position whose
+ * page is not in the table or not in [0, n_pages) is not written; with check != 0 the
+ * call synchronizes and reports it as CATNN_ERR_SHAPE. No two rows may name
+ * the same slot (two sequences that share a page append to it apart). */
+int catnn_kv_append(catnn_ctx* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                    int64_t v_stride, const float* wq, const float* wk, void* q_out, void* k_cache, void* v_cache,
+                    const int32_t* page_table, const int32_t* seq_lens, const int32_t* cu_tokens, int64_t tokens,
+                    int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd, int64_t n_pages, int64_t page_size,
+                    int64_t max_pages, double theta, float eps, int dtype, int check);
+
+/* Attention of one new token of each sequence, the last of its seq_lens[i]
+ * cached positions: q [seqs, n_heads, hd] -> o [seqs, n_heads*hd] and lse
+ * fp32 [seqs, n_heads], with the scale, head grouping and window of
+ * catnn_attention_fwd. A sequence of length 0 (or less) gets o = 0 and lse =
+ * -inf. Slots past a sequence's end and before its window are never used,
+ * whatever they hold. hd at most 128. Positions on a page that is not in
+ * [0, n_pages), or beyond the table, are left out; with check != 0 the call
+ * synchronizes and reports them as CATNN_ERR_SHAPE. */
+int catnn_paged_attention_workspace(catnn_ctx* ctx, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd,
+                                    size_t* bytes);
+int catnn_paged_attention_fwd(catnn_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache,
+                              const void* v_cache, const int32_t* page_table, const int32_t* seq_lens, void* o,
+                              float* lse, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd, int64_t n_pages,
+                              int64_t page_size, int64_t max_pages, int64_t window, int dtype, void* workspace,
+                              size_t workspace_bytes, int check);
+
+/* catnn_moe_fwd for at most CATNN_MOE_FEW_MAX_TOKENS rows of x: the same
+ * block (router ties to the lower index, E <= 32) in two kernels that read
+ * each chosen expert's weights once, with no padding of experts to 128 rows. */
+#define CATNN_MOE_FEW_MAX_TOKENS 64
+int catnn_moe_few_workspace(catnn_ctx* ctx, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k, int dtype,
+                            size_t* bytes);
+int catnn_moe_few_fwd(catnn_ctx* ctx, const void* x, const void* gate, const void* w1s, const void* w3s,
+                      const void* w2s, void* y, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k,
+                      int dtype, void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------ optimizers */
 /* p -= lr·g (Sgd::put, crates/catnn-core/src/lens/optim.rs:32). fp32
  * master; shadow_bf16 (optional) receives bf16(p). */

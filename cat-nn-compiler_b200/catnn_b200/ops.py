@@ -26,24 +26,27 @@ class Context:
         h = C.c_void_p()
         _lib.call("catnn_ctx_create", int(device), C.byref(h))
         self.handle = h
+        self._stream = None
         self._workspace = {}
 
     def bind(self):
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
+        s = torch._C._cuda_getCurrentRawStream(self.device)
+        if s != self._stream:
+            _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
+            self._stream = s
         return self.handle
 
     def workspace(self, name, *sizes):
-        """A workspace of the bytes that `name`'s _workspace function asks
-        for, from torch's allocator (so it belongs to the current stream, or
-        to the graph being captured), or None where it asks for none. The
-        sizes asked for are kept, not the memory."""
+        """(workspace, bytes) that `name`'s _workspace function asks for, from
+        torch's allocator (so it belongs to the current stream, or to the
+        graph being captured); (None, 0) where it asks for none. The size is
+        kept, not the memory."""
         n = self._workspace.get((name, sizes))
         if n is None:
             v = C.c_size_t()
             _lib.call(name, self.handle, *sizes, C.byref(v))
             n = self._workspace[(name, sizes)] = int(v.value)
-        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        return (torch.empty(n, dtype=torch.uint8, device=self.device), n) if n else (None, 0)
 
     def launch_count(self):
         v = C.c_uint64()
@@ -529,13 +532,17 @@ def moe_backward(x, gate, w1s, w3s, w2s, dy, top_k):
 
 
 # ------------------------------------------------------------------ decoding
+# A decoding step calls these with next to nothing to compute, so what the
+# host spends on a call counts: shapes are unpacked once and compared as numbers.
 def _on(t, *others):
-    """All of one call's tensors lie on one CUDA device."""
-    if not t.is_cuda:
+    """All of one call's tensors lie on one CUDA device; its context."""
+    d = t.get_device()
+    if d < 0:
         raise InvalidArgument("catnn_b200 operators take CUDA tensors")
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != d:
             raise InvalidArgument(f"tensors on {t.device} and {o.device}")
+    return _CTX.get(d) or context(d)
 
 
 def _rows(t, what):
@@ -543,22 +550,22 @@ def _rows(t, what):
     dense and whose tokens evenly spaced: a tensor of its own, or a column
     block of the rows that one QKV product writes."""
     *lead, heads, hd = t.shape
-    st = t.stride()
+    *st, per_head, per_value = t.stride()
     if t.numel() == 0:
         return heads * hd
-    if (hd > 1 and st[-1] != 1) or (heads > 1 and st[-2] != hd):
+    if (hd > 1 and per_value != 1) or (heads > 1 and per_head != hd):
         raise InvalidArgument(f"{what}: a token's heads must be dense")
-    step = None  # stride of the next inner token dimension, times its size
-    for n, s in zip(reversed(lead), reversed(st[:-2])):
+    token, span = heads * hd, None  # span: stride of the next outer dimension that is evenly spaced
+    while lead:
+        n, step = lead.pop(), st.pop()
         if n == 1:
             continue
-        if step is None:
-            token, step = s, s * n
-        elif s != step:
+        if span is None:
+            token = step
+        elif step != span:
             raise InvalidArgument(f"{what}: tokens must be evenly spaced")
-        else:
-            step = s * n
-    return heads * hd if step is None else token
+        span = step * n
+    return token
 
 
 def _i32(t, what):
@@ -572,19 +579,26 @@ def _i32(t, what):
 def _weight(w, hd, what):
     if w.dtype != torch.float32:
         raise DTypeMismatch(f"{what} must be float32")
-    if w.shape != (hd,) or (hd > 1 and w.stride(0) != 1):
+    if w.numel() != hd or w.dim() != 1 or not w.is_contiguous():
         raise ShapeMismatch(f"{what} must be a dense [{hd}] vector")
     return w.data_ptr()
 
 
-def _qk(q, k, wq, wk, positions, what):
+def _qk(q, k, what):
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
+        raise ShapeMismatch(f"{what}: q {tuple(qs)}, k {tuple(ks)}")
     _same(q, k)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ShapeMismatch(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}")
-    if positions is not None and positions.shape != q.shape[:2]:
+    b, s, h, hd = qs
+    return b, s, h, ks[2], hd
+
+
+def _positions(positions, b, s, what):
+    if positions is None:
+        return None
+    if tuple(positions.shape) != (b, s):
         raise ShapeMismatch(f"{what}: positions {tuple(positions.shape)}")
-    _on(q, k, wq, wk, positions)
-    return None if positions is None else _i32(positions, "positions")
+    return _i32(positions, "positions")
 
 
 def qk_norm_rope(q, k, wq, wk, theta, eps=1e-5, positions=None):
@@ -592,12 +606,11 @@ def qk_norm_rope(q, k, wq, wk, theta, eps=1e-5, positions=None):
     weights wq, wk [hd] (fp32), then the rotation of its pairs to its position,
     in one pass -> (q', k'), dense. positions int32 [B,S]; None: 0..S-1. q and k
     may be column blocks of packed QKV rows."""
-    pos = _qk(q, k, wq, wk, positions, "qk_norm_rope")
-    b, s, h, hd = q.shape
-    hkv = k.shape[2]
-    qo = torch.empty((b, s, h, hd), dtype=q.dtype, device=q.device)
-    ko = torch.empty((b, s, hkv, hd), dtype=q.dtype, device=q.device)
-    _lib.call("catnn_qk_norm_rope_fwd", _h(q), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
+    b, s, h, hkv, hd = _qk(q, k, "qk_norm_rope")
+    pos = _positions(positions, b, s, "qk_norm_rope")
+    ctx = _on(q, k, wq, wk, positions)
+    qo, ko = q.new_empty((b, s, h, hd)), k.new_empty((b, s, hkv, hd))
+    _lib.call("catnn_qk_norm_rope_fwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
               _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, qo.data_ptr(), ko.data_ptr(), b, s, h, hkv, hd, theta, eps,
               _dt(q))
     return qo, ko
@@ -606,37 +619,33 @@ def qk_norm_rope(q, k, wq, wk, theta, eps=1e-5, positions=None):
 def qk_norm_rope_backward(q, k, wq, wk, dq_out, dk_out, theta, eps=1e-5, positions=None):
     """Adjoint of qk_norm_rope from its inputs and the gradients of its
     results -> (dq, dk, dwq, dwk); dwq and dwk are summed in a fixed order."""
-    _same(q, dq_out, dk_out)
+    b, s, h, hkv, hd = _qk(q, k, "qk_norm_rope backward")
+    pos = _positions(positions, b, s, "qk_norm_rope backward")
     if dq_out.shape != q.shape or dk_out.shape != k.shape:
         raise ShapeMismatch(f"qk_norm_rope backward: dq_out {tuple(dq_out.shape)}, dk_out {tuple(dk_out.shape)}")
-    pos = _qk(q, k, wq, wk, positions, "qk_norm_rope backward")
-    _on(q, dq_out, dk_out)
-    b, s, h, hd = q.shape
-    hkv = k.shape[2]
-    ctx = context(q.device)
-    ws = ctx.workspace("catnn_qk_norm_rope_bwd_workspace", b, s, h, hkv, hd)
-    dq = torch.empty((b, s, h, hd), dtype=q.dtype, device=q.device)
-    dk = torch.empty((b, s, hkv, hd), dtype=q.dtype, device=q.device)
-    dw = torch.empty((2, hd), dtype=torch.float32, device=q.device)
+    _same(q, dq_out, dk_out)
+    ctx = _on(q, k, wq, wk, positions, dq_out, dk_out)
+    ws, n = ctx.workspace("catnn_qk_norm_rope_bwd_workspace", b, s, h, hkv, hd)
+    dq, dk, dw = q.new_empty((b, s, h, hd)), k.new_empty((b, s, hkv, hd)), wq.new_empty((2, hd))
+    dwq, dwk = dw.unbind()
     _lib.call("catnn_qk_norm_rope_bwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
               _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, dq_out.data_ptr(), _rows(dq_out, "dq_out"),
-              dk_out.data_ptr(), _rows(dk_out, "dk_out"), dq.data_ptr(), dk.data_ptr(), dw.data_ptr(),
-              dw.data_ptr() + 4 * hd, b, s, h, hkv, hd, theta, eps, _dt(q), None if ws is None else ws.data_ptr(),
-              0 if ws is None else ws.numel())
-    return dq, dk, dw[0], dw[1]
+              dk_out.data_ptr(), _rows(dk_out, "dk_out"), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+              b, s, h, hkv, hd, theta, eps, _dt(q), ws.data_ptr() if n else None, n)
+    return dq, dk, dwq, dwk
 
 
 def _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, like, what):
+    """Checks a paged cache -> (pages, page size), (sequences, table columns), table, lengths."""
+    ks, ts = k_cache.shape, page_table.shape
+    if len(ks) != 4 or v_cache.shape != ks or ks[1] != hkv or ks[3] != hd:
+        raise ShapeMismatch(f"{what}: caches {tuple(ks)}, {tuple(v_cache.shape)} for {hkv} heads of {hd}")
+    if len(ts) != 2 or seq_lens.dim() != 1 or seq_lens.numel() != ts[0]:
+        raise ShapeMismatch(f"{what}: page table {tuple(ts)}, lengths {tuple(seq_lens.shape)}")
     _same(like, k_cache, v_cache)
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != hkv or k_cache.shape[3] != hd:
-        raise ShapeMismatch(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} for {hkv} heads of {hd}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise InvalidArgument(f"{what}: caches must be contiguous")
-    if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0]:
-        raise ShapeMismatch(f"{what}: page table {tuple(page_table.shape)}, lengths {tuple(seq_lens.shape)}")
-    ptrs = _i32(page_table, "page_table"), _i32(seq_lens, "seq_lens")
-    _on(like, k_cache, v_cache, page_table, seq_lens)
-    return ptrs
+    return (ks[0], ks[2]), ts, _i32(page_table, "page_table"), _i32(seq_lens, "seq_lens")
 
 
 def kv_append(q, k, v, k_cache, v_cache, page_table, seq_lens, theta, cu_tokens=None, wq=None, wk=None, eps=1e-5,
@@ -653,27 +662,35 @@ def kv_append(q, k, v, k_cache, v_cache, page_table, seq_lens, theta, cu_tokens=
     zero); slots without a page are not written, which check=True
     (synchronizing) reports as a ShapeMismatch. No two rows may name the same
     slot."""
-    if k.dim() != 3 or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0]
-                                                                 or q.shape[2] != k.shape[2])):
-        raise ShapeMismatch(f"kv_append: q {None if q is None else tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    t, hkv, hd = k.shape
-    h = 0 if q is None else q.shape[1]
-    seqs = page_table.shape[0]
+    ks = k.shape
+    if len(ks) != 3 or v.shape != ks:
+        raise ShapeMismatch(f"kv_append: k {tuple(ks)}, v {tuple(v.shape)}")
+    t, hkv, hd = ks
+    (pages, page), (seqs, most), table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, k, "kv_append")
     _same(k, v, q)
-    if cu_tokens is not None and cu_tokens.shape != (seqs + 1,):
-        raise ShapeMismatch(f"kv_append: cu_tokens {tuple(cu_tokens.shape)} for {seqs} sequences")
+    h, qo, qp, q_rows, qop = 0, None, None, 0, None
+    if q is not None:
+        qs = q.shape
+        if len(qs) != 3 or qs[0] != t or qs[2] != hd:
+            raise ShapeMismatch(f"kv_append: q {tuple(qs)}, k {tuple(ks)}")
+        h, qp, q_rows = qs[1], q.data_ptr(), _rows(q, "q")
+    cu = None
+    if cu_tokens is not None:
+        if cu_tokens.dim() != 1 or cu_tokens.numel() != seqs + 1:
+            raise ShapeMismatch(f"kv_append: cu_tokens {tuple(cu_tokens.shape)} for {seqs} sequences")
+        cu = _i32(cu_tokens, "cu_tokens")
+    elif t != seqs:
+        raise ShapeMismatch(f"kv_append: {t} rows for {seqs} sequences without cu_tokens")
     if (wq is None) != (wk is None):
         raise InvalidArgument("kv_append: both norm weights or neither")
-    if cu_tokens is None and t != seqs:
-        raise ShapeMismatch(f"kv_append: {t} rows for {seqs} sequences without cu_tokens")
-    table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, k, "kv_append")
-    _on(k, q, v, cu_tokens, wq, wk)
-    qo = None if q is None else torch.empty((t, h, hd), dtype=q.dtype, device=q.device)
-    _lib.call("catnn_kv_append", _h(k), None if q is None else q.data_ptr(), 0 if q is None else _rows(q, "q"),
-              k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), None if wq is None else _weight(wq, hd, "wq"),
-              None if wk is None else _weight(wk, hd, "wk"), None if q is None else qo.data_ptr(), k_cache.data_ptr(),
-              v_cache.data_ptr(), table, lens, None if cu_tokens is None else _i32(cu_tokens, "cu_tokens"), t, seqs, h, hkv,
-              hd, k_cache.shape[0], k_cache.shape[2], page_table.shape[1], theta, eps, _dt(k), int(check))
+    wqp, wkp = (None, None) if wq is None else (_weight(wq, hd, "wq"), _weight(wk, hd, "wk"))
+    ctx = _on(k, q, v, k_cache, v_cache, page_table, seq_lens, cu_tokens, wq, wk)
+    if q is not None:
+        qo = q.new_empty((t, h, hd))
+        qop = qo.data_ptr()
+    _lib.call("catnn_kv_append", ctx.bind(), qp, q_rows, k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), wqp, wkp,
+              qop, k_cache.data_ptr(), v_cache.data_ptr(), table, lens, cu, t, seqs, h, hkv, hd, pages, page, most, theta, eps,
+              _dt(k), check)
     return qo
 
 
@@ -682,21 +699,20 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, window=None, chec
     cached positions, the last of which is its own (append first)
     -> (o [seqs,H*hd], lse [seqs,H]). Caches, table and lengths as in
     kv_append; a sequence of length 0 gets zeros and -inf."""
-    if q.dim() != 3:
-        raise ShapeMismatch(f"paged_attention: q {tuple(q.shape)}")
-    b, h, hd = q.shape
-    hkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    if hkv < 1 or h % hkv or seq_lens.shape[0] != b:
-        raise ShapeMismatch(f"paged_attention: q {tuple(q.shape)} for {hkv} kv heads, {tuple(seq_lens.shape)} sequences")
-    table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, q, "paged_attention")
-    ctx = context(q.device)
-    ws = ctx.workspace("catnn_paged_attention_workspace", b, h, hkv, hd)
-    o = torch.empty((b, h * hd), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, h), dtype=torch.float32, device=q.device)
+    qs, ks = q.shape, k_cache.shape
+    hkv = ks[1] if len(ks) == 4 else 0
+    if len(qs) != 3 or hkv < 1 or qs[1] % hkv:
+        raise ShapeMismatch(f"paged_attention: q {tuple(qs)} for {hkv} kv heads")
+    b, h, hd = qs
+    (pages, page), (seqs, most), table, lens = _cache(k_cache, v_cache, page_table, seq_lens, hkv, hd, q, "paged_attention")
+    if seqs != b:
+        raise ShapeMismatch(f"paged_attention: {b} queries, {seqs} sequences")
+    ctx = _on(q, k_cache, v_cache, page_table, seq_lens)
+    ws, n = ctx.workspace("catnn_paged_attention_workspace", b, h, hkv, hd)
+    o, lse = q.new_empty((b, h * hd)), q.new_empty((b, h), dtype=torch.float32)
     _lib.call("catnn_paged_attention_fwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(),
-              table, lens, o.data_ptr(), lse.data_ptr(), b, h, hkv, hd, k_cache.shape[0], k_cache.shape[2],
-              page_table.shape[1], int(window or 0), _dt(q), None if ws is None else ws.data_ptr(),
-              0 if ws is None else ws.numel(), int(check))
+              table, lens, o.data_ptr(), lse.data_ptr(), b, h, hkv, hd, pages, page, most, window or 0, _dt(q),
+              ws.data_ptr() if n else None, n, check)
     return o, lse
 
 
@@ -704,27 +720,26 @@ def moe_few(x, gate, w1s, w3s, w2s, top_k):
     """moe() for at most 64 rows of x, in two kernels that read each chosen
     expert's weights once; expert weights stacked [E, ...]."""
     _same(x, gate, w1s, w3s, w2s)
+    ws1 = w1s.shape
     hid = x.shape[-1]
-    t = x.numel() // max(hid, 1)
-    if w1s.dim() != 3:
-        raise ShapeMismatch(f"moe_few: w1s {tuple(w1s.shape)}")
-    e, _, mid = w1s.shape
-    if (w1s.shape != (e, hid, mid) or w3s.shape != w1s.shape or w2s.shape != (e, mid, hid) or gate.shape != (hid, e)):
-        raise ShapeMismatch(f"moe_few: x {tuple(x.shape)}, gate {tuple(gate.shape)}, w1s {tuple(w1s.shape)}, "
-                            f"w3s {tuple(w3s.shape)}, w2s {tuple(w2s.shape)}")
+    if len(ws1) != 3 or ws1[1] != hid:
+        raise ShapeMismatch(f"moe_few: x {tuple(x.shape)}, w1s {tuple(ws1)}")
+    e, _, mid = ws1
+    if w3s.shape != ws1 or tuple(w2s.shape) != (e, mid, hid) or tuple(gate.shape) != (hid, e):
+        raise ShapeMismatch(f"moe_few: gate {tuple(gate.shape)}, w1s {tuple(ws1)}, w3s {tuple(w3s.shape)}, "
+                            f"w2s {tuple(w2s.shape)}")
     if not (x.is_contiguous() and gate.is_contiguous() and w1s.is_contiguous() and w3s.is_contiguous()
             and w2s.is_contiguous()):
         raise InvalidArgument("catnn_b200 operators take contiguous tensors")
+    t = x.numel() // max(hid, 1)
     if t > 64 or not 1 <= top_k <= e <= 32:
         raise ShapeMismatch(f"moe_few: {t} rows (at most 64), top {top_k} of {e} experts (at most 32)")
     dt = _dt(x)
-    _on(x, gate, w1s, w3s, w2s)
-    ctx = context(x.device)
-    ws = ctx.workspace("catnn_moe_few_workspace", t, hid, mid, e, top_k, dt)
+    ctx = _on(x, gate, w1s, w3s, w2s)
+    ws, n = ctx.workspace("catnn_moe_few_workspace", t, hid, mid, e, top_k, dt)
     y = torch.empty_like(x)
     _lib.call("catnn_moe_few_fwd", ctx.bind(), x.data_ptr(), gate.data_ptr(), w1s.data_ptr(), w3s.data_ptr(),
-              w2s.data_ptr(), y.data_ptr(), t, hid, mid, e, top_k, dt, None if ws is None else ws.data_ptr(),
-              0 if ws is None else ws.numel())
+              w2s.data_ptr(), y.data_ptr(), t, hid, mid, e, top_k, dt, ws.data_ptr() if n else None, n)
     return y
 
 

@@ -812,6 +812,22 @@ CUtensorMap tma_map_bf16(const void* base, i64 rows, i64 cols, i64 ld, int box_c
     return make_map(base, rows, cols, ld, box_cols, box_rows);
 }
 
+CUtensorMap tma_map_stack(const void* base, i64 planes, i64 rows, i64 cols, int dtype, int box_cols, int box_rows) {
+    CUtensorMap m;
+    const bool b16 = dtype == CATNN_BF16;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)cols * dsize(dtype), (cuuint64_t)(rows * cols) * dsize(dtype)};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = encode_fn()(&m, b16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+                             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             !b16 ? CU_TENSOR_MAP_SWIZZLE_NONE : box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                               : CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CATNN_CHECK(r == CUDA_SUCCESS, CATNN_ERR_CUDA, "cuTensorMapEncodeTiled (stack) failed (" + std::to_string((int)r) + ")");
+    return m;
+}
+
 template <bool A_MN, bool B_MN, int BN, int STAGES, bool TF32 = false>
 static void launch_tc(Context* c, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc,
                       const CUtensorMap& md, const TcArgs& a, int grid) {

@@ -75,7 +75,7 @@ SIGNATURES = {
                                I64, F64, F32, I32, VP, C.c_size_t],
     "catnn_kv_append": [VP, VP, I64, VP, I64, VP, I64, VP, VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I64,
                         I64, I64, F64, F32, I32, I32],
-    "catnn_paged_attention_workspace": [VP, I64, I64, I64, I64, C.POINTER(C.c_size_t)],
+    "catnn_paged_attention_workspace": [VP, I64, I64, I64, I64, I32, C.POINTER(C.c_size_t)],
     "catnn_paged_attention_fwd": [VP, VP, I64, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I64, I64, I64, I32, VP,
                                   C.c_size_t, I32],
     "catnn_moe_few_workspace": [VP, I64, I64, I64, I64, I64, I32, C.POINTER(C.c_size_t)],

@@ -126,12 +126,15 @@ int catnn_kv_append(catnn_ctx* h, const void* q, int64_t q_stride, const void* k
     ABI_END
 }
 
-int catnn_paged_attention_workspace(catnn_ctx* h, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd, size_t* bytes) {
+int catnn_paged_attention_workspace(catnn_ctx* h, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd, int dtype,
+                                    size_t* bytes) {
     ABI_BEGIN
     Context* c = unwrap(h);
+    check_dtype(dtype);
     need(bytes, "bytes");
     heads_ok(seqs, 1, n_heads, n_kv, hd, "paged_attention");
-    *bytes = paged_attention_workspace(c, seqs, n_heads, n_kv, hd);
+    shape(n_heads % n_kv == 0, "paged_attention: n_heads must be a multiple of n_kv");
+    *bytes = paged_attention_workspace(c, seqs, n_heads, n_kv, hd, dtype);
     ABI_END
 }
 
@@ -152,7 +155,7 @@ int catnn_paged_attention_fwd(catnn_ctx* h, const void* q, int64_t q_stride, con
     need(max_pages == 0 || n_pages == 0 || (k_cache && v_cache && page_table), "k_cache/v_cache/page_table");
     stride_ok(q_stride, seqs, n_heads * hd, "paged_attention q");
     if (window <= 0 || window > INT_MAX) window = 0;  // none, or longer than any table's positions
-    workspace_ok(workspace, workspace_bytes, paged_attention_workspace(c, seqs, n_heads, n_kv, hd), "paged_attention");
+    workspace_ok(workspace, workspace_bytes, paged_attention_workspace(c, seqs, n_heads, n_kv, hd, dtype), "paged_attention");
     paged_attention(c, q, q_stride, k_cache, v_cache, page_table, seq_lens, o, lse, seqs, n_heads, n_kv, hd, n_pages, page_size,
                     n_pages == 0 ? 0 : max_pages, window, dtype, workspace, flag(c, check, SLOT_PAGED));
     if (check && take_status(c, SLOT_PAGED))

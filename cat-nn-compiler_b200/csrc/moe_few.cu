@@ -194,8 +194,9 @@ __device__ __forceinline__ unsigned choose(float l, int E, int k, int lane, floa
     return taken;
 }
 
-template <int R8, int CW>
-__device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, char* gs, float* part) {
+// `issued` is called by every warp when its first batch's loads are on their way.
+template <int R8, int CW, typename Issued>
+__device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, char* gs, float* part, Issued issued) {
     constexpr int NB = R8 == 1 ? 8 : 4;  // runs of 32 k in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, kj = (lane & 3) * 8;
     const int nt = (a.E + 7) / 8, ep = nt * 8;
@@ -225,9 +226,11 @@ __device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, cha
 #pragma unroll
                 for (int q = 0; q < NB; ++q)
                     g[q] = k0 + q * CW * 32 + lane < a.hidden ? *(const uint4*)(grow + q * CW * 32 * a.E) : make_uint4(0, 0, 0, 0);
+                if (j == 0 && k0 == warp * 32) issued();
 #pragma unroll
                 for (int q = 0; q < NB; ++q) *(uint4*)(gs + q * 512 + lane * 16) = g[q];
             } else {
+                if (j == 0 && k0 == warp * 32) issued();
                 unsigned short* to = (unsigned short*)(gs + lane * 16);
 #pragma unroll 1
                 for (int q = 0; q < NB; ++q)
@@ -286,18 +289,34 @@ template <bool ALL, int CW> __device__ __forceinline__ void find_expert(const Tc
     }
 }
 
-template <int R8, int CW>
-__device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r) {
+// Fills r.taken, and the weights: `w` in shared memory where it is not null, or
+// with `tell`, `taken` and the weights in the workspace. `prefetch` is run by
+// the copying warp as soon as the loads of x and the gate are under way (before
+// them it would hold them up in the memory's queues).
+template <int R8, int CW, typename Prefetch>
+__device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r, float* w_here, bool tell, Prefetch prefetch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cl = cg::this_cluster();
     const int shares = (a.T + RT - 1) / RT, mine = shares > 1 ? (int)cl.block_rank() : 0;
     const int t0 = mine * RT, rows = min(RT, a.T - t0), ep = (a.E + 7) / 8 * 8;  // rows below 1: none of its own
-    if (shares > 1) cl.barrier_arrive();  // waited for below: a peer's memory may be written once it has started
+    // waited for below: a peer's memory may be written once it has started
+    if (shares > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     float* part = (float*)room;           // [CW][RT][ep], then the warps' gate rows
-    if (warp < CW && rows > 0) logits_tc<R8, CW>(a, t0, rows, room + CW * RT * MAX_E * 4, part);
-    if (shares > 1) cl.barrier_wait();
+    const auto issued = [] { asm volatile("bar.arrive 1, %0;" ::"n"((CW + 1) * 32) : "memory"); };
+    if (warp == CW) {
+        asm volatile("bar.sync 1, %0;" ::"n"((CW + 1) * 32) : "memory");
+        prefetch();
+    } else if (rows > 0 && warp * 32 < a.hidden) {
+        logits_tc<R8, CW>(a, t0, rows, room + CW * RT * MAX_E * 4, part, issued);
+    } else {
+        issued();
+        for (int i = lane; i < RT * ep; i += 32) part[warp * RT * ep + i] = 0.f;
+    }
+    if (shares > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     __syncthreads();
-    const int peers = shares > 1 ? (int)cl.num_blocks() : 1;
+    unsigned* to = r.taken;  // lane p's copy of it
+    if (shares > 1) to = cl.map_shared_rank(r.taken, min(lane, (int)cl.num_blocks() - 1));
+    const int copies = shares > 1 ? (int)cl.num_blocks() : 1;
 #pragma unroll 1
     for (int i = warp; i < rows; i += CW + 1) {
         float l = 0.f, top;
@@ -305,16 +324,18 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r)
 #pragma unroll
             for (int w = 0; w < CW; ++w) l += part[(w * RT + i) * ep + lane];
         const unsigned taken = choose(l, a.E, a.k, lane, top);
-        const bool in = taken >> lane & 1u;
-        float w = in ? __expf(l - top) : 0.f;
-        w *= 1.f / fmaxf(warp_sum(w), 1e-30f);
-        const int t = t0 + i, at = t * a.k + __popc(taken & ((1u << lane) - 1u));
-#pragma unroll 1
-        for (int p = 0; p < peers; ++p) {
-            unsigned* pt = shares > 1 ? cl.map_shared_rank(r.taken, p) : r.taken;
-            float* pw = shares > 1 ? cl.map_shared_rank(r.w, p) : r.w;
-            if (lane == 0) pt[t] = taken;
-            if (in) pw[at] = w;
+        const int t = t0 + i;
+        if (lane < copies) to[t] = taken;
+        if (w_here || tell) {
+            const bool in = taken >> lane & 1u;
+            float w = in ? __expf(l - top) : 0.f;
+            w = __fdividef(w, fmaxf(warp_sum(w), 1e-30f));
+            const int at = t * a.k + __popc(taken & ((1u << lane) - 1u));
+            if (in && w_here) w_here[at] = w;
+            if (tell) {
+                if (in) ((float*)(a.taken + a.T))[at] = w;
+                if (lane == 0) a.taken[t] = taken;
+            }
         }
     }
     tc::fence_proxy_async();  // `part` and the gate rows lie where TMA writes next
@@ -367,8 +388,12 @@ template <bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
                 tc::mbar_init(&empty[s], CW);
             }
             tc::fence_mbar_init();
-            for (int it = 0; it < PRE && it < iters; ++it) weights(it, it, blockIdx.z);
         }
+    }
+    // The slot's first tiles, by the copying warp.
+    __device__ __forceinline__ void prefetch() const {
+        if (threadIdx.x == CW * 32)
+            for (int it = 0; it < PRE && it < iters; ++it) weights(it, it, blockIdx.z);
     }
     __device__ __forceinline__ void weights(int it, int st, int expert) const {
         char* at = ring + st * W_BYTES;
@@ -512,9 +537,8 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
     if (first)
         for (int i = threadIdx.x; i < (a.hidden + 63) / 64; i += S::THREADS) a.count[i] = 0u;
-    route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring + S::PRE * S::W_BYTES, r);
-    if (ALL && first)
-        for (int i = threadIdx.x; i < a.T * (a.k + 1); i += S::THREADS) a.taken[i] = r.taken[i];  // w follows
+    route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring + S::PRE * S::W_BYTES, r, nullptr,
+                                  ALL && blockIdx.x < cg::this_cluster().dim_blocks().x && blockIdx.z == 0, [&] { s.prefetch(); });
     find_expert<ALL, CW>(a, blockIdx.z, r);
     if (r.n == 0) {  // the whole cluster: it shares its slot
         s.drain(a);
@@ -554,11 +578,12 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     using S = Tc<ALL, 1, NT, BN, CW, ROOM>;
     const S s(a, raw, r, &w2, &w2, a.down_run, a.mid, a.hidden);
     if (ALL) {
+        s.prefetch();
         tc::grid_dependency_wait();
         for (int i = threadIdx.x; i < a.T * (a.k + 1); i += S::THREADS) r.taken[i] = __ldcg(a.taken + i);
         __syncthreads();
     } else {
-        route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring, r);
+        route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring, r, r.w, false, [] {});
     }
     find_expert<ALL, CW>(a, blockIdx.z, r);
     if (r.n == 0) {
@@ -585,30 +610,46 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     __syncthreads();
     if (!last) return;
     __threadfence();
-    constexpr int Q = BN / 4;
+    // four tokens at a time, so that their loads are in flight together
+    constexpr int Q = BN / 4, AT_ONCE = 4;
+    const int c = col0 + threadIdx.x % Q * 4;
+    if (c >= a.hidden) return;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < a.T * Q; i += S::THREADS) {
-        const int t = i / Q, c = col0 + (i - t * Q) * 4;
-        if (c >= a.hidden) continue;
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
-        const float* p = a.yp + (i64)t * a.k * a.hidden + c;
-        for (int j = 0; j < a.k; ++j, p += a.hidden) {
-            const float w = r.w[t * a.k + j];
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int q = 0; q < (int)gridDim.y; ++q) {
-                const float4 u = __ldcg((const float4*)(p + q * run_size));
-                v.x += u.x;
-                v.y += u.y;
-                v.z += u.z;
-                v.w += u.w;
+    for (int tb = threadIdx.x / Q; tb < a.T; tb += S::THREADS / Q * AT_ONCE) {
+        float4 y[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int j = 0; j < a.k; ++j) {
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int q = 0; q < (int)gridDim.y; ++q)
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const int t = min(tb + i * (S::THREADS / Q), a.T - 1);
+                    const float4 u = __ldcg((const float4*)(a.yp + q * run_size + ((i64)t * a.k + j) * a.hidden + c));
+                    v[i].x += u.x;
+                    v[i].y += u.y;
+                    v[i].z += u.z;
+                    v[i].w += u.w;
+                }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float w = r.w[min(tb + i * (S::THREADS / Q), a.T - 1) * a.k + j];
+                y[i].x = fmaf(w, v[i].x, y[i].x);
+                y[i].y = fmaf(w, v[i].y, y[i].y);
+                y[i].z = fmaf(w, v[i].z, y[i].z);
+                y[i].w = fmaf(w, v[i].w, y[i].w);
             }
-            y[0] = fmaf(w, v.x, y[0]);
-            y[1] = fmaf(w, v.y, y[1]);
-            y[2] = fmaf(w, v.z, y[2]);
-            y[3] = fmaf(w, v.w, y[3]);
         }
-        stv<bf16, 4>(a.y + (i64)t * a.hidden + c, y);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int t = tb + i * (S::THREADS / Q);
+            const float o[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+            if (t < a.T) stv<bf16, 4>(a.y + (i64)t * a.hidden + c, o);
+        }
     }
 }
 
@@ -683,8 +724,8 @@ template <typename F> static void with_shape(Context* c, i64 T, i64 mid, i64 slo
     else if (T <= 8) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
     else if (T <= 16 && thin) f(Shape<false, 2, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
     else if (T <= 16) f(Shape<false, 2, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
-    else if (T <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 68 * K, 3>());
-    else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 68 * K, 3>());
+    else if (T <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+    else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
 }
 
 // Where things lie in the workspace of the tensor-core kernels.

@@ -221,7 +221,7 @@ void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_str
                const float* wq, const float* wk, void* qo, void* kc, void* vc, const int32_t* table, const int32_t* lens,
                const int32_t* cu, i64 tokens, i64 seqs, i64 h, i64 hkv, i64 hd, i64 pages, i64 page, i64 max_pages,
                double theta, float eps, int dtype, int* err);
-size_t paged_attention_workspace(Context* c, i64 seqs, i64 h, i64 hkv, i64 hd);
+size_t paged_attention_workspace(Context* c, i64 seqs, i64 h, i64 hkv, i64 hd, int dtype);
 void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, const void* vc, const int32_t* table,
                      const int32_t* lens, void* o, float* lse, i64 seqs, i64 h, i64 hkv, i64 hd, i64 pages, i64 page,
                      i64 max_pages, i64 window, int dtype, void* work, int* err);

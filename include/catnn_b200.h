@@ -342,7 +342,7 @@ int catnn_kv_append(catnn_ctx* ctx, const void* q, int64_t q_stride, const void*
  * [0, n_pages), or beyond the table, are left out; with check != 0 the call
  * synchronizes and reports them as CATNN_ERR_SHAPE. */
 int catnn_paged_attention_workspace(catnn_ctx* ctx, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd,
-                                    size_t* bytes);
+                                    int dtype, size_t* bytes);
 int catnn_paged_attention_fwd(catnn_ctx* ctx, const void* q, int64_t q_stride, const void* k_cache,
                               const void* v_cache, const int32_t* page_table, const int32_t* seq_lens, void* o,
                               float* lse, int64_t seqs, int64_t n_heads, int64_t n_kv, int64_t hd, int64_t n_pages,

@@ -15,6 +15,7 @@
 // that it shares with others goes to the workspace, and a second, dependent
 // kernel joins those in order; a (sequence, head) of one warp is written at once.
 #include <algorithm>
+#include <climits>
 #include <mutex>
 #include <set>
 
@@ -42,7 +43,6 @@ struct Args {
     int* err;
     // tiles: a sequence's segments are its kv heads times the tiles of `rows` query heads of a group
     int rows, row_tiles, workers, pitch;  // pitch: floats of a row in `part`
-    i64* prefix;                          // [seqs + 1] tiles before a sequence
     float *part, *ml;                     // [workers][2][rows][pitch] sums, [workers][2][rows][2] maximum and weight
 };
 
@@ -58,64 +58,67 @@ __device__ __forceinline__ int tiles_of(const Args& a, i64 b) {  // of one segme
     return (len - first + TK - 1) / TK;
 }
 
-__device__ __forceinline__ i64 warp_sum64(i64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-__device__ __forceinline__ i64 warp_scan64(i64 v, int lane) {  // inclusive
+__device__ __forceinline__ int warp_sum_int(int v) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)v); }
+__device__ __forceinline__ int warp_scan_int(int v, int lane) {  // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const i64 u = __shfl_up_sync(0xffffffffu, v, o);
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
     return v;
 }
 
-// Warps that take part, and the first tile of warp w of them: N tiles dealt out evenly.
-__device__ __forceinline__ i64 workers_of(const Args& a, i64 n) { return min((i64)a.workers, (n + MIN_TILES - 1) / MIN_TILES); }
-
-// Tiles of all sequences; their sums by chunks of sequences in shared memory.
+// Tiles of all sequences (the host sees to it that they stay below 2^31) and
+// how they are dealt out: `workers` warps take `each` tiles in a row, the
+// first `more` one more. Up to 32 sequences a lane keeps its one's tiles;
+// of more, shared memory the sums of chunks of them.
 struct Count {
-    i64 total;
-    int per, chunks;
-};
-template <int W> __device__ __forceinline__ Count count_tiles(const Args& a, i64* chunk) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const i64 segs = (i64)a.hkv * a.row_tiles;
-    Count c;
-    c.per = (int)max((i64)32, (a.seqs + MAX_CHUNKS - 1) / MAX_CHUNKS);
-    c.chunks = (int)((a.seqs + c.per - 1) / c.per);
-    for (int i = warp; i < c.chunks; i += W) {
-        const i64 b1 = min(a.seqs, (i64)(i + 1) * c.per);
-        i64 s = 0;
-        for (i64 b = (i64)i * c.per + lane; b < b1; b += 32) s += tiles_of(a, b) * segs;
-        s = warp_sum64(s);
-        if (lane == 0) chunk[i] = s;
+    int total, per, chunks, workers, each, more;
+    int own;  // this lane's sequence's tiles, where there are no more than 32
+    __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
+    __device__ __forceinline__ int worker(int tile) const {  // the one that has it
+        const int big = more * (each + 1);
+        return tile < big ? tile / (each + 1) : more + (tile - big) / each;
     }
-    __syncthreads();
-    i64 s = 0;
-    for (int i = lane; i < c.chunks; i += 32) s += chunk[i];
-    c.total = warp_sum64(s);
+};
+template <int W> __device__ __forceinline__ Count count_tiles(const Args& a, int* chunk) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, segs = a.hkv * a.row_tiles;
+    Count c;
+    if (a.seqs <= 32) {
+        c.per = c.chunks = 0;
+        c.own = lane < a.seqs ? tiles_of(a, lane) * segs : 0;
+        c.total = warp_sum_int(c.own);
+    } else {
+        c.per = (int)max((i64)32, (a.seqs + MAX_CHUNKS - 1) / MAX_CHUNKS);
+        c.chunks = (int)((a.seqs + c.per - 1) / c.per);
+        for (int i = warp; i < c.chunks; i += W) {
+            const i64 b1 = min(a.seqs, (i64)(i + 1) * c.per);
+            int s = 0;
+            for (i64 b = (i64)i * c.per + lane; b < b1; b += 32) s += tiles_of(a, b) * segs;
+            s = warp_sum_int(s);
+            if (lane == 0) chunk[i] = s;
+        }
+        __syncthreads();
+        int s = 0;
+        for (int i = lane; i < c.chunks; i += 32) s += chunk[i];
+        c.own = 0;
+        c.total = warp_sum_int(s);
+    }
+    c.workers = max(1, min(a.workers, (c.total + MIN_TILES - 1) / MIN_TILES));
+    c.each = c.total / c.workers;
+    c.more = c.total - c.each * c.workers;
     return c;
 }
 
-// The tiles before each sequence, for the joining kernel: by one CTA.
-template <int W> __device__ __forceinline__ void write_prefix(const Args& a, const Count& c, const i64* chunk) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const i64 segs = (i64)a.hkv * a.row_tiles;
-    for (int i = warp; i < c.chunks; i += W) {
-        i64 at = 0;
-        for (int j = lane; j < i; j += 32) at += chunk[j];
-        at = warp_sum64(at);
-        const i64 b1 = min(a.seqs, (i64)(i + 1) * c.per);
-        for (i64 b0 = (i64)i * c.per; b0 < b1; b0 += 32) {
-            const i64 b = b0 + lane, n = b < b1 ? tiles_of(a, b) * segs : 0, up = warp_scan64(n, lane);
-            if (b < b1) a.prefix[b] = at + up - n;
-            at += __shfl_sync(0xffffffffu, up, 31);
-        }
-    }
-    if (threadIdx.x == 0) a.prefix[a.seqs] = c.total;
+// The tiles before sequence b, by a warp.
+__device__ __forceinline__ int tiles_before(const Args& a, const Count& c, const int* chunk, i64 b) {
+    const int lane = threadIdx.x & 31, segs = a.hkv * a.row_tiles;
+    if (c.chunks == 0) return warp_sum_int(lane < b ? c.own : 0);
+    const int in = (int)(b / c.per);
+    int s = 0;
+    for (int i = lane; i < in; i += 32) s += chunk[i];
+    for (i64 x = (i64)in * c.per + lane; x < b; x += 32) s += tiles_of(a, x) * segs;
+    return warp_sum_int(s);
 }
 
 // A place in the order of tiles: sequence, segment (kv head major, then row
@@ -140,74 +143,89 @@ struct At {
     }
 };
 // Where tile t is (0 <= t < total).
-__device__ __forceinline__ At locate(const Args& a, const Count& c, const i64* chunk, i64 t) {
+__device__ __forceinline__ At locate(const Args& a, const Count& c, const int* chunk, int t) {
     const int lane = threadIdx.x & 31, segs = a.hkv * a.row_tiles;
-    int i = 0;
-    for (; i < c.chunks; i += 32) {  // the chunk
-        const i64 n = i + lane < c.chunks ? chunk[i + lane] : 0, up = warp_scan64(n, lane);
-        const unsigned past = __ballot_sync(0xffffffffu, up > t);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            t -= __shfl_sync(0xffffffffu, up - n, l);
-            i += l;
-            break;
-        }
-        t -= __shfl_sync(0xffffffffu, up, 31);
-    }
     At at;
     at.b = a.seqs;
     at.seg = at.tile = at.tiles = at.first = at.len = 0;
-    const i64 b1 = min(a.seqs, (i64)(i + 1) * c.per);
-    for (i64 b0 = (i64)i * c.per; b0 < b1; b0 += 32) {  // the sequence
-        const i64 b = b0 + lane, n = b < b1 ? (i64)tiles_of(a, b) * segs : 0, up = warp_scan64(n, lane);
+    // the first of 32 counts, one a lane, that reaches past t, which becomes the rest: its lane, or -1
+    auto reach = [&](int n) {
+        const int up = warp_scan_int(n, lane);
         const unsigned past = __ballot_sync(0xffffffffu, up > t);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            t -= __shfl_sync(0xffffffffu, up - n, l);
-            at.b = b0 + l;
-            break;
+        const int l = past ? __ffs(past) - 1 : 31;
+        t -= __shfl_sync(0xffffffffu, past ? up - n : up, l);
+        return past ? l : -1;
+    };
+    if (c.chunks == 0) {
+        const int l = reach(c.own);
+        if (l >= 0) at.b = l;
+    } else {
+        int i = 0, l = -1;
+        for (; i < c.chunks && l < 0; i += l < 0 ? 32 : 0) {
+            l = reach(i + lane < c.chunks ? chunk[i + lane] : 0);
+            if (l >= 0) i += l;
         }
-        t -= __shfl_sync(0xffffffffu, up, 31);
+        const i64 b1 = min(a.seqs, (i64)(i + 1) * c.per);
+        l = -1;
+        for (i64 b0 = (i64)i * c.per; b0 < b1 && l < 0; b0 += 32) {
+            l = reach(b0 + lane < b1 ? tiles_of(a, b0 + lane) * segs : 0);
+            if (l >= 0) at.b = b0 + l;
+        }
     }
     if (at.b >= a.seqs) return at;  // lengths that changed under the kernel: nothing to do, but no way astray
     at.enter(a);
     if (at.tiles == 0) return at;
-    at.seg = (int)(t / at.tiles);
-    at.tile = (int)(t - (i64)at.seg * at.tiles);
+    at.seg = t / at.tiles;
+    at.tile = t - at.seg * at.tiles;
     return at;
 }
 
 // What a warp does with its tiles, whatever the type of the cache: a ring of
 // S tiles of K and V rows, each row of hd values at a pitch of PITCH bytes
 // (an odd number of 16-byte pieces: neither ldmatrix nor row-a-lane reads meet
-// bank conflicts). Lane l looks up where row l of the tile to come lies, one
-// tile ahead; rows without a position or a page are zeros and not in `mask`.
+// bank conflicts). Lane l looks up where row l of a tile lies, two
+// tiles before it is fetched; rows without a position or a page are zeros and not in `mask`.
 template <typename T, int HDP, int S> struct Ring {
     static constexpr int PITCH = HDP * (int)sizeof(T) + 16, VEC = 16 / (int)sizeof(T), PIECES = HDP / VEC;
     static constexpr int TILE = TK * PITCH, STAGE = 2 * TILE, BYTES = S * STAGE + 16 * ((S * 4 + 15) / 16);
     char* base;
     unsigned* mask;
-    At at;        // the tile to fetch next
-    i64 left;     // tiles still to fetch
-    int slot, id; // this lane's row of it: slot of its page, page (below 0: no position)
+    At at;         // the tile to look up next
+    int look_left, left;  // tiles still to look up, to fetch
+    // this lane's row of the next two tiles to fetch: kv head, slot of its page, page (-2: no position)
+    int kvh[2], slot[2], id[2];
 
     __device__ __forceinline__ void look(const Args& a) {
-        const int pos = at.first + at.tile * TK + (threadIdx.x & 31);
-        id = -2;
-        slot = 0;
-        if (left > 0 && pos < at.len) {
-            const int p = (unsigned)pos / (unsigned)a.page;
-            slot = pos - p * a.page;
-            id = a.table[at.b * a.max_pages + p];
+        kvh[0] = kvh[1], slot[0] = slot[1], id[0] = id[1];
+        id[1] = -2;
+        if (look_left > 0) {
+            const int pos = at.first + at.tile * TK + (threadIdx.x & 31);
+            kvh[1] = at.seg / a.row_tiles;
+            if (pos < at.len) {
+                const int p = (unsigned)pos / (unsigned)a.page;
+                slot[1] = pos - p * a.page;
+                id[1] = a.table[at.b * a.max_pages + p];
+            }
+            --look_left;
+            at.next(a, a.hkv * a.row_tiles);
+            if (at.tiles == 0) look_left = 0;
         }
+    }
+    __device__ __forceinline__ void start(const Args& a, const At& first, int tiles) {
+        at = first;
+        look_left = left = tiles;
+        kvh[1] = slot[1] = 0;
+        look(a);
+        look(a);
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) fetch(a, s);
     }
     __device__ __forceinline__ void fetch(const Args& a, int stage) {
         const int lane = threadIdx.x & 31;
         if (left > 0) {
-            const bool on = id >= 0 && id < a.pages;
-            if (a.err && !on && id != -2) atomicExch(a.err, 1);
-            const int kvh = at.seg / a.row_tiles;
-            const i64 off = on ? (((i64)id * a.hkv + kvh) * a.page + slot) * a.hd : -1;
+            const bool on = id[0] >= 0 && id[0] < a.pages;
+            if (a.err && !on && id[0] != -2) atomicExch(a.err, 1);
+            const i64 off = on ? (((i64)id[0] * a.hkv + kvh[0]) * a.page + slot[0]) * a.hd : -1;
             const unsigned m = __ballot_sync(0xffffffffu, on);
             if (lane == 0) mask[stage] = m;
             const uint32_t to = tc::smem_u32(base + stage * STAGE);
@@ -221,8 +239,6 @@ template <typename T, int HDP, int S> struct Ring {
                 tc::cp_async16(to + TILE + row * PITCH + c * 16, (const T*)a.vc + e, here);
             }
             --left;
-            at.next(a, a.hkv * a.row_tiles);
-            if (at.tiles == 0) left = 0;
             look(a);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -247,12 +263,12 @@ struct Dest {
     i64 slot;   // row 0 of its slot in part / ml
     int rows;   // heads of this row tile
 };
-__device__ __forceinline__ Dest dest_of(const Args& a, const At& seg, i64 worker, bool first, bool whole) {
+__device__ __forceinline__ Dest dest_of(const Args& a, const At& seg, int worker, bool first, bool whole) {
     const int group = a.h / a.hkv, kvh = seg.seg / a.row_tiles, r0 = (seg.seg - kvh * a.row_tiles) * a.rows;
     Dest d;
     d.rows = min(a.rows, group - r0);
     d.out = whole ? seg.b * a.h + kvh * group + r0 : -1;
-    d.slot = (worker * 2 + (first ? 0 : 1)) * a.rows;
+    d.slot = ((i64)worker * 2 + (first ? 0 : 1)) * a.rows;
     return d;
 }
 
@@ -266,31 +282,27 @@ __global__ void __launch_bounds__(W * 32) k_paged_mma(const __grid_constant__ Ar
     using R = Ring<bf16, HDP, S>;
     constexpr int KS = HDP / 16, NV = HDP / 8;
     extern __shared__ __align__(16) char raw[];
-    __shared__ i64 chunk[MAX_CHUNKS];
+    __shared__ int chunk[MAX_CHUNKS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, segs = a.hkv * a.row_tiles;
     tc::launch_dependents();
     const Count c = count_tiles<W>(a, chunk);
-    if (blockIdx.x == 0) write_prefix<W>(a, c, chunk);
-    const i64 workers = workers_of(a, c.total), me = (i64)warp * gridDim.x + blockIdx.x;  // few warps: one an SM first
-    if (me >= workers) return;
-    const i64 t0 = me * c.total / workers, t1 = (me + 1) * c.total / workers;
+    const int me = warp * gridDim.x + blockIdx.x;  // few warps: one an SM first
+    if (me >= c.workers || c.total == 0) return;
+    const int t0 = c.start(me), t1 = c.start(me + 1);
     R ring;
     ring.base = raw + warp * R::BYTES;
     ring.mask = (unsigned*)(ring.base + S * R::STAGE);
-    ring.left = t1 - t0;
-    At cur = ring.at = locate(a, c, chunk, t0);
+    At cur = locate(a, c, chunk, t0);
     if (cur.tiles == 0) return;
-    ring.look(a);
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) ring.fetch(a, s);
+    ring.start(a, cur, t1 - t0);
     const float sc = a.scale * LOG2E;
     const uint32_t kaddr = (lane & 7) * R::PITCH + (lane >> 3) * 16;
     const uint32_t vaddr = ((lane & 7) + (lane >> 3 & 1) * 8) * R::PITCH + (lane >> 4) * 16;
     bool first = true;
     int stage = 0;
-    for (i64 t = t0; t < t1 && cur.tiles > 0;) {
+    for (int t = t0; t < t1 && cur.tiles > 0;) {
         // a segment, or this warp's part of it
-        const int here = (int)min((i64)(cur.tiles - cur.tile), t1 - t);
+        const int here = min(cur.tiles - cur.tile, t1 - t);
         const Dest d = dest_of(a, cur, me, first, here == cur.tiles);
         uint32_t qa[KS][R8 * 2];
         {
@@ -425,37 +437,37 @@ __global__ void __launch_bounds__(W * 32) k_paged_mma(const __grid_constant__ Ar
 // ------------------------------------------------------------ fp32: FMA
 // A lane has a position's scores for the first product and hd / 32 columns
 // for the second; q and the weights pass through shared memory, from where
-// whole warps read the same words.
+// whole warps read the same words. Shared memory's wavefronts bound it, so
+// everything moves in the widest pieces there are.
+template <int N> struct __align__(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) Floats {
+    float v[N];
+};
 template <int HDP, int G, int S, int W>
 __global__ void __launch_bounds__(W * 32) k_paged_fma(const __grid_constant__ Args a) {
     using R = Ring<float, HDP, S>;
     constexpr int C = HDP / 32;
     constexpr int WARP_BYTES = R::BYTES + G * (HDP + TK) * 4;
     extern __shared__ __align__(16) char raw[];
-    __shared__ i64 chunk[MAX_CHUNKS];
+    __shared__ int chunk[MAX_CHUNKS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, segs = a.hkv * a.row_tiles;
     tc::launch_dependents();
     const Count c = count_tiles<W>(a, chunk);
-    if (blockIdx.x == 0) write_prefix<W>(a, c, chunk);
-    const i64 workers = workers_of(a, c.total), me = (i64)warp * gridDim.x + blockIdx.x;
-    if (me >= workers) return;
-    const i64 t0 = me * c.total / workers, t1 = (me + 1) * c.total / workers;
+    const int me = warp * gridDim.x + blockIdx.x;
+    if (me >= c.workers || c.total == 0) return;
+    const int t0 = c.start(me), t1 = c.start(me + 1);
     R ring;
     ring.base = raw + warp * WARP_BYTES;
     ring.mask = (unsigned*)(ring.base + S * R::STAGE);
     float* const qs = (float*)(ring.base + R::BYTES);  // [HDP / 4][G][4]
     float* const ps = qs + G * HDP;                    // [TK][G]
-    ring.left = t1 - t0;
-    At cur = ring.at = locate(a, c, chunk, t0);
+    At cur = locate(a, c, chunk, t0);
     if (cur.tiles == 0) return;
-    ring.look(a);
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) ring.fetch(a, s);
+    ring.start(a, cur, t1 - t0);
     const float sc = a.scale * LOG2E;
     bool first = true;
     int stage = 0;
-    for (i64 t = t0; t < t1 && cur.tiles > 0;) {
-        const int here = (int)min((i64)(cur.tiles - cur.tile), t1 - t);
+    for (int t = t0; t < t1 && cur.tiles > 0;) {
+        const int here = min(cur.tiles - cur.tile, t1 - t);
         const Dest d = dest_of(a, cur, me, first, here == cur.tiles);
         {
             const int group = a.h / a.hkv, kvh = cur.seg / a.row_tiles, r0 = (cur.seg - kvh * a.row_tiles) * a.rows;
@@ -491,6 +503,7 @@ __global__ void __launch_bounds__(W * 32) k_paged_fma(const __grid_constant__ Ar
                     s[g] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[g]))));
                 }
             }
+            Floats<G> pw;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 if (!(mask >> lane & 1u)) s[g] = -INFINITY;
@@ -501,21 +514,19 @@ __global__ void __launch_bounds__(W * 32) k_paged_fma(const __grid_constant__ Ar
 #pragma unroll
                     for (int u = 0; u < C; ++u) o[g][u] *= keep;
                 m[g] = top;
-                ps[lane * G + g] = p;
+                pw.v[g] = p;
             }
+            *(Floats<G>*)(ps + lane * G) = pw;
             __syncwarp();
             const char* vb = kb + R::TILE + lane * C * 4;
 #pragma unroll 4
             for (int j = 0; j < TK; ++j) {
-                float v[C];
+                const Floats<C> v = *(const Floats<C>*)(vb + j * R::PITCH);
+                const Floats<G> p = *(const Floats<G>*)(ps + j * G);
 #pragma unroll
-                for (int u = 0; u < C; ++u) v[u] = *(const float*)(vb + j * R::PITCH + u * 4);
+                for (int g = 0; g < G; ++g)
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float p = ps[j * G + g];
-#pragma unroll
-                    for (int u = 0; u < C; ++u) o[g][u] = fmaf(p, v[u], o[g][u]);
-                }
+                    for (int u = 0; u < C; ++u) o[g][u] = fmaf(p.v[g], v.v[u], o[g][u]);
             }
             __syncwarp();
             if (++stage == S) stage = 0;
@@ -545,77 +556,88 @@ __global__ void __launch_bounds__(W * 32) k_paged_fma(const __grid_constant__ Ar
 }
 
 // ------------------------------------------------------------ join
-// A CTA to a (sequence, query head): nothing to do where one warp had all of
-// it; zeros and -inf where there is nothing to attend to; else the parts of
-// the warps that shared it, each brought to the largest maximum. Threads take
-// four columns, and several of them, by turns, the parts.
-constexpr int JOIN = 256;
-template <typename T>
-__global__ void __launch_bounds__(JOIN) k_paged_join(const __grid_constant__ Args a) {
-    __shared__ float4 sum[JOIN];
-    __shared__ float weight[JOIN], red[32];
-    tc::grid_dependency_wait();
-    const int segs = a.hkv * a.row_tiles, tid = threadIdx.x, group = a.h / a.hkv;
-    const int quads = (a.hd + 3) / 4, turns = JOIN / quads, quad = tid / turns, turn = tid - quad * turns;
+// A CTA to a (sequence, query head) and the next one a grid on: nothing to do
+// where one warp had all of it; zeros and -inf where there is nothing to
+// attend to; else the parts of the warps that shared it, each brought to the
+// largest maximum. Threads take four columns, and several of them, by turns,
+// the parts. Who shared what is found out while the first kernel still runs.
+// Few heads can have many parts each: 512 threads to one then, 128 otherwise,
+// so that the CTAs find their places while the first kernel still runs.
+template <typename T, int JOIN>
+__global__ void __launch_bounds__(JOIN, 1280 / JOIN) k_paged_join(const __grid_constant__ Args a) {
+    __shared__ int chunk[MAX_CHUNKS];
+    const int segs = a.hkv * a.row_tiles, tid = threadIdx.x, group = a.h / a.hkv, quads = (a.hd + 3) / 4;
+    int turns = JOIN / 32;  // a power of two: the threads of four columns lie in one warp
+    while (turns < 32 && 2 * turns * quads <= JOIN) turns *= 2;
+    const int quad = tid / turns, turn = tid & (turns - 1);
+    const Count c = count_tiles<JOIN / 32>(a, chunk);
+    bool waited = false;
     for (i64 out = blockIdx.x; out < a.seqs * a.h; out += gridDim.x) {
         const i64 b = out / a.h;
         const int head = (int)(out - b * a.h), kvh = head / group, rt = (head - kvh * group) / a.rows;
-        const int row = head - kvh * group - rt * a.rows;
-        const i64 p0 = __ldcg(a.prefix + b), total = __ldcg(a.prefix + a.seqs);
-        const i64 tiles = (__ldcg(a.prefix + b + 1) - p0) / segs, s = p0 + (kvh * a.row_tiles + rt) * tiles, e = s + tiles;
+        const int row = head - kvh * group - rt * a.rows, tiles = tiles_of(a, b);
         if (a.err && tid == 0 && a.lens[b] > (i64)a.max_pages * a.page) atomicExch(a.err, 1);
         if (tiles == 0) {
             for (int i = tid; i < a.hd; i += JOIN) st((T*)a.o + out * a.hd + i, 0.f);
             if (tid == 0) a.lse[out] = -INFINITY;
             continue;
         }
-        const i64 workers = workers_of(a, total);
-        // warp w starts at tile floor(w·total / workers): the last one to start at or before a tile
-        const i64 w0 = ((s + 1) * workers - 1) / total, w1 = (e * workers - 1) / total;
+        const int s = tiles_before(a, c, chunk, b) + (kvh * a.row_tiles + rt) * tiles, w0 = c.worker(s), w1 = c.worker(s + tiles - 1);
         if (w0 == w1) continue;
-        const int parts = (int)(w1 - w0 + 1);
-        const i64 slot0 = (w0 * 2 + (w0 * total / workers < s ? 1 : 0)) * a.rows + row;  // the others start here: their first slot
-        auto slot_of = [&](int p) { return p ? (w0 + p) * 2 * a.rows + row : slot0; };
-        float top = -INFINITY;
-        for (int p = tid; p < parts; p += JOIN) top = fmaxf(top, __ldcg(a.ml + slot_of(p) * 2));
-        top = block_max(top, red);
-        const float base = top == -INFINITY ? 0.f : top;
-        float w = 0.f;
+        const int parts = w1 - w0 + 1;
+        // the first may have come here from another segment; the others start here
+        const i64 slot0 = ((i64)w0 * 2 + (c.start(w0) < s ? 1 : 0)) * a.rows + row;
+        if (!waited) {
+            tc::grid_dependency_wait();
+            waited = true;
+        }
+        float m = -INFINITY, w = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (quad < quads)
-#pragma unroll 4
-            for (int p = turn; p < parts; p += turns) {
-                const i64 slot = slot_of(p);
-                const float2 ml = __ldcg((const float2*)(a.ml + slot * 2));
-                const float4 u = __ldcg((const float4*)(a.part + slot * a.pitch + quad * 4));
-                const float f = ex2(ml.x - base);
-                w = fmaf(f, ml.y, w);
-                v.x = fmaf(f, u.x, v.x);
-                v.y = fmaf(f, u.y, v.y);
-                v.z = fmaf(f, u.z, v.z);
-                v.w = fmaf(f, u.w, v.w);
+            for (int p0 = turn; p0 < parts; p0 += 4 * turns) {
+                float2 ml[4];
+                float4 u[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int p = p0 + i * turns;
+                    const i64 slot = p ? (i64)(w0 + p) * 2 * a.rows + row : slot0;
+                    ml[i] = p < parts ? __ldcg((const float2*)(a.ml + slot * 2)) : make_float2(-INFINITY, 0.f);
+                    u[i] = p < parts ? __ldcg((const float4*)(a.part + slot * a.pitch + quad * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), base = top == -INFINITY ? 0.f : top;
+                float f = ex2(m - base);
+                w *= f;
+                v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                m = top;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f = ex2(ml[i].x - base);
+                    w = fmaf(f, ml[i].y, w);
+                    v.x = fmaf(f, u[i].x, v.x);
+                    v.y = fmaf(f, u[i].y, v.y);
+                    v.z = fmaf(f, u[i].z, v.z);
+                    v.w = fmaf(f, u[i].w, v.w);
+                }
             }
-        sum[tid] = v;
-        weight[tid] = w;
-        __syncthreads();
+        for (int o = 1; o < turns; o <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), w2 = __shfl_xor_sync(0xffffffffu, w, o);
+            const float4 v2 = make_float4(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o),
+                                          __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o));
+            const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top, f = ex2(m - base), f2 = ex2(m2 - base);
+            m = top;
+            w = w * f + w2 * f2;
+            v = make_float4(v.x * f + v2.x * f2, v.y * f + v2.y * f2, v.z * f + v2.z * f2, v.w * f + v2.w * f2);
+        }
         if (quad < quads && turn == 0) {
-            for (int u = 1; u < min(turns, parts); ++u) {
-                const float4 x = sum[tid + u];
-                w += weight[tid + u];
-                v.x += x.x;
-                v.y += x.y;
-                v.z += x.z;
-                v.w += x.w;
-            }
             const float inv = w == 0.f ? 0.f : 1.f / w;
             const float r[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (quad * 4 + u < a.hd) st((T*)a.o + out * a.hd + quad * 4 + u, w == 0.f ? 0.f : r[u]);
-            if (quad == 0) a.lse[out] = w == 0.f ? -INFINITY : LN2 * (top + log2f(w));
+            if (quad == 0) a.lse[out] = w == 0.f ? -INFINITY : LN2 * (m + log2f(w));
         }
-        __syncthreads();
     }
+    if (!waited) tc::grid_dependency_wait();  // what comes after this kernel comes after the first one too
 }
 
 // ------------------------------------------------------------ any size and alignment
@@ -690,23 +712,22 @@ struct Fill {
 static Fill fill_of(int dtype, int hd, int group) {
     if (dtype == CATNN_BF16) return hd <= 64 ? Fill{4, 2, group <= 8 ? 8 : 16} : Fill{4, 1, group <= 8 ? 8 : 16};
     const int rows = group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
-    return hd <= 96 ? Fill{4, 1, rows} : Fill{3, 1, rows};
+    return Fill{hd <= 96 ? 4 : 3, 1, rows};
 }
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct Layout {
-    size_t part, ml, bytes;
+    size_t ml, bytes;
     int workers, rows, pitch;
 };
-static Layout layout(Context* c, i64 seqs, i64 h, i64 hkv, i64 hd, int dtype) {
+static Layout layout(Context* c, i64 h, i64 hkv, i64 hd, int dtype) {
     const Fill f = fill_of(dtype, (int)hd, (int)(h / hkv));
     Layout l;
     l.workers = c->sm_count * f.per_sm * f.warps;
     l.rows = (int)std::min<i64>(f.rows, h / hkv);
     l.pitch = (int)((hd + 3) / 4 * 4);
-    l.part = align256((size_t)(seqs + 1) * 8);
-    l.ml = l.part + align256((size_t)l.workers * 2 * l.rows * l.pitch * 4);
+    l.ml = align256((size_t)l.workers * 2 * l.rows * l.pitch * 4);
     l.bytes = l.ml + align256((size_t)l.workers * 2 * l.rows * 2 * 4);
     return l;
 }
@@ -740,18 +761,18 @@ template <int G> static void run_fma_hd(Context* c, const Args& a, const Fill& f
 
 using namespace paged;
 
-size_t paged_attention_workspace(Context* c, i64 seqs, i64 h, i64 hkv, i64 hd, int dtype) {
-    return layout(c, seqs, h, hkv, hd, dtype).bytes;
+size_t paged_attention_workspace(Context* c, i64, i64 h, i64 hkv, i64 hd, int dtype) {
+    return layout(c, h, hkv, hd, dtype).bytes;
 }
 
 void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, const void* vc, const int32_t* table,
                      const int32_t* lens, void* o, float* lse, i64 seqs, i64 h, i64 hkv, i64 hd, i64 pages, i64 page,
                      i64 max_pages, i64 window, int dtype, void* work, int* err) {
     if (seqs == 0) return;
-    const Layout l = layout(c, seqs, h, hkv, hd, dtype);
+    const Layout l = layout(c, h, hkv, hd, dtype);
     Args a{q, kc, vc, o, lse, table, lens, seqs, (int)h, (int)hkv, (int)hd, (int)page, (int)max_pages, (int)window, pages,
-           q_stride, 1.0f / sqrtf((float)hd), err, l.rows, cdiv(h / hkv, l.rows), l.workers, l.pitch, (i64*)work,
-           (float*)((char*)work + l.part), (float*)((char*)work + l.ml)};
+           q_stride, 1.0f / sqrtf((float)hd), err, l.rows, cdiv(h / hkv, l.rows), l.workers, l.pitch, (float*)work,
+           (float*)((char*)work + l.ml)};
     const int vec = dtype == CATNN_BF16 ? 8 : 4;
     if (hd % vec != 0 || !aligned_to(kc, 16) || !aligned_to(vc, 16) || !aligned_to(q, 4) || (seqs > 1 && q_stride % 2 != 0) ||
         !aligned_to(o, 4)) {
@@ -760,6 +781,9 @@ void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, co
         launched(c);
         return;
     }
+    const i64 most = max_pages * page, reach = window > 0 ? std::min(most, window) : most;
+    CATNN_CHECK(seqs * hkv * a.row_tiles <= INT_MAX / (reach / TK + 2), CATNN_ERR_UNSUPPORTED,
+                "paged_attention: the table's positions times the heads pass 2^31 tiles of 32");
     const Fill f = fill_of(dtype, (int)hd, (int)(h / hkv));
     if (dtype == CATNN_BF16) {
         const bool eight = f.rows == 8;
@@ -773,17 +797,18 @@ void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, co
         else if (f.rows == 4) run_fma_hd<4>(c, a, f);
         else run_fma_hd<8>(c, a, f);
     }
+    const bool few = seqs * h <= 2 * c->sm_count;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::min<i64>(seqs * h, 65536));
-    cfg.blockDim = dim3(JOIN);
+    cfg.gridDim = dim3((unsigned)std::min<i64>(seqs * h, (i64)c->sm_count * 10));
+    cfg.blockDim = dim3(few ? 512 : 128);
     cfg.stream = c->stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (dtype == CATNN_BF16) CUDA_OK(cudaLaunchKernelEx(&cfg, k_paged_join<bf16>, a));
-    else CUDA_OK(cudaLaunchKernelEx(&cfg, k_paged_join<float>, a));
+    if (dtype == CATNN_BF16) CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<bf16, 512> : k_paged_join<bf16, 128>, a));
+    else CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<float, 512> : k_paged_join<float, 128>, a));
     launched(c);
 }
 

@@ -561,15 +561,17 @@ __global__ void __launch_bounds__(W * 32) k_paged_fma(const __grid_constant__ Ar
 // attend to; else the parts of the warps that shared it, each brought to the
 // largest maximum. Threads take four columns, and several of them, by turns,
 // the parts. Who shared what is found out while the first kernel still runs.
-// Few heads can have many parts each: 512 threads to one then, 128 otherwise,
+// Few heads can have many parts each: 256 threads to one then, 128 otherwise,
 // so that the CTAs find their places while the first kernel still runs.
 template <typename T, int JOIN>
-__global__ void __launch_bounds__(JOIN, 1280 / JOIN) k_paged_join(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(JOIN, JOIN == 128 ? 10 : 3) k_paged_join(const __grid_constant__ Args a) {
     __shared__ int chunk[MAX_CHUNKS];
     const int segs = a.hkv * a.row_tiles, tid = threadIdx.x, group = a.h / a.hkv, quads = (a.hd + 3) / 4;
-    int turns = JOIN / 32;  // a power of two: the threads of four columns lie in one warp
-    while (turns < 32 && 2 * turns * quads <= JOIN) turns *= 2;
-    const int quad = tid / turns, turn = tid & (turns - 1);
+    __shared__ float4 sum[JOIN / 32][MAX_HD / 4];
+    __shared__ float2 weight[JOIN / 32][MAX_HD / 4];
+    const int lane = tid & 31, warp = tid >> 5;
+    const int lq = quads <= 8 ? 8 : quads <= 16 ? 16 : 32;  // lanes that take a part's row together
+    const int quad = lane & (lq - 1), turns = JOIN / lq, turn = tid / lq;
     const Count c = count_tiles<JOIN / 32>(a, chunk);
     bool waited = false;
     for (i64 out = blockIdx.x; out < a.seqs * a.h; out += gridDim.x) {
@@ -619,16 +621,23 @@ __global__ void __launch_bounds__(JOIN, 1280 / JOIN) k_paged_join(const __grid_c
                     v.w = fmaf(f, u[i].w, v.w);
                 }
             }
-        for (int o = 1; o < turns; o <<= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), w2 = __shfl_xor_sync(0xffffffffu, w, o);
-            const float4 v2 = make_float4(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o),
-                                          __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o));
+        auto add = [&](float m2, float w2, float4 v2) {
             const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top, f = ex2(m - base), f2 = ex2(m2 - base);
             m = top;
             w = w * f + w2 * f2;
             v = make_float4(v.x * f + v2.x * f2, v.y * f + v2.y * f2, v.z * f + v2.z * f2, v.w * f + v2.w * f2);
+        };
+        for (int o = lq; o < 32; o <<= 1)
+            add(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, w, o),
+                make_float4(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o),
+                            __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o)));
+        if (warp > 0 && lane < quads) {
+            sum[warp][lane] = v;
+            weight[warp][lane] = make_float2(m, w);
         }
-        if (quad < quads && turn == 0) {
+        __syncthreads();
+        if (warp == 0 && lane < quads) {
+            for (int u = 1; u < JOIN / 32; ++u) add(weight[u][lane].x, weight[u][lane].y, sum[u][lane]);
             const float inv = w == 0.f ? 0.f : 1.f / w;
             const float r[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
 #pragma unroll
@@ -636,6 +645,7 @@ __global__ void __launch_bounds__(JOIN, 1280 / JOIN) k_paged_join(const __grid_c
                 if (quad * 4 + u < a.hd) st((T*)a.o + out * a.hd + quad * 4 + u, w == 0.f ? 0.f : r[u]);
             if (quad == 0) a.lse[out] = w == 0.f ? -INFINITY : LN2 * (m + log2f(w));
         }
+        __syncthreads();
     }
     if (!waited) tc::grid_dependency_wait();  // what comes after this kernel comes after the first one too
 }
@@ -800,15 +810,15 @@ void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, co
     const bool few = seqs * h <= 2 * c->sm_count;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::min<i64>(seqs * h, (i64)c->sm_count * 10));
-    cfg.blockDim = dim3(few ? 512 : 128);
+    cfg.blockDim = dim3(few ? 256 : 128);
     cfg.stream = c->stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (dtype == CATNN_BF16) CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<bf16, 512> : k_paged_join<bf16, 128>, a));
-    else CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<float, 512> : k_paged_join<float, 128>, a));
+    if (dtype == CATNN_BF16) CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<bf16, 256> : k_paged_join<bf16, 128>, a));
+    else CUDA_OK(cudaLaunchKernelEx(&cfg, few ? k_paged_join<float, 256> : k_paged_join<float, 128>, a));
     launched(c);
 }
 

@@ -19,6 +19,7 @@
 
 #include "ops.cuh"
 #include "paged_place.cuh"
+#include "tc_prims.cuh"
 
 namespace catnn {
 namespace qkn {
@@ -83,53 +84,79 @@ struct FwdArgs {
     i64 tokens, s;
     int h, hkv, hd;
     float eps;
-    // a warp takes `per` row groups of a token, `units` warps a token
+    // a unit is up to `per` row groups of a token, `units` units a token
     int per, units;
 };
 
+// 16 bytes as V values.
+template <typename T, int V> __device__ __forceinline__ void unpack(const uint4& r, float (&o)[V]) {
+    if constexpr (sizeof(T) == 4) {
+        o[0] = __uint_as_float(r.x), o[1] = __uint_as_float(r.y), o[2] = __uint_as_float(r.z), o[3] = __uint_as_float(r.w);
+    } else {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[2 * j] = __uint_as_float(w[j] << 16);
+            o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+    }
+}
+
 // Forward on 16-byte pieces. Group g of a token holds heads
-// [g·HPW, (g+1)·HPW) of its H query heads followed by its Hkv key heads.
+// [g·HPW, (g+1)·HPW) of its H query heads followed by its Hkv key heads. A
+// warp walks the units in grid order; all rows of a unit are on their way
+// before its sines are taken.
+constexpr int UNIT = 6;  // row groups of a unit, at most
 template <typename T, int LPH>
-__global__ void __launch_bounds__(WARPS * 32) k_qk_fwd(const __grid_constant__ FwdArgs a, const __grid_constant__ Freq f) {
+__global__ void __launch_bounds__(WARPS * 32, 3) k_qk_fwd(const __grid_constant__ FwdArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
-    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V;
-    const i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const i64 tok = unit / a.units;
-    if (tok >= a.tokens) return;
-    const int g0 = (int)(unit - tok * a.units) * a.per, heads = a.h + a.hkv;
-    const int g1 = min(g0 + a.per, (heads + HPW - 1) / HPW);
+    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V, heads = a.h + a.hkv;
     const bool in = e0 < a.hd;
     float wq[V], wk[V];
-    float2 cs[V / 2];
-    const int p = a.pos ? a.pos[tok] : (int)(tok % a.s);
 #pragma unroll
     for (int u = 0; u < V; ++u) wq[u] = wk[u] = 0.f;
     if (in) {
         ldv<float, V>(a.wq + e0, wq);
         ldv<float, V>(a.wk + e0, wk);
-#pragma unroll
-        for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
     }
-    const T* qrow = (const T*)a.q + tok * a.q_stride;
-    const T* krow = (const T*)a.k + tok * a.k_stride;
-    T* qo = (T*)a.qo + tok * a.h * a.hd;
-    T* ko = (T*)a.ko + tok * a.hkv * a.hd;
-    for (int g = g0; g < g1; ++g) {
-        const int head = g * HPW + sub;
-        const bool isq = head < a.h, on = in && head < heads;
-        float x[V];
+    const i64 all = a.tokens * a.units;
+    for (i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += (i64)gridDim.x * WARPS) {
+        const i64 tok = a.units == 1 ? unit : unit / a.units;
+        const int head0 = (int)(unit - tok * a.units) * a.per * HPW + sub;
+        const T* qrow = (const T*)a.q + tok * a.q_stride + e0;
+        const T* krow = (const T*)a.k + tok * a.k_stride + e0;
+        uint4 raw[UNIT];
 #pragma unroll
-        for (int u = 0; u < V; ++u) x[u] = 0.f;
-        if (on) ldv<T, V>((isq ? qrow + (i64)head * a.hd : krow + (i64)(head - a.h) * a.hd) + e0, x);
-        float ss = 0.f;
+        for (int g = 0; g < UNIT; ++g) {
+            const int head = head0 + g * HPW;
+            raw[g] = make_uint4(0, 0, 0, 0);
+            if (g < a.per && in && head < heads)
+                raw[g] = *(const uint4*)(head < a.h ? qrow + (i64)head * a.hd : krow + (i64)(head - a.h) * a.hd);
+        }
+        const int p = a.pos ? a.pos[tok] : (int)(tok % a.s);
+        float2 cs[V / 2];
+        if (in)
 #pragma unroll
-        for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
-        const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
-        if (!on) continue;
+            for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
+        T* qo = (T*)a.qo + tok * a.h * a.hd + e0;
+        T* ko = (T*)a.ko + tok * a.hkv * a.hd + e0;
 #pragma unroll
-        for (int u = 0; u < V; ++u) x[u] = x[u] * r * (isq ? wq[u] : wk[u]);
-        rotate<V>(x, cs);
-        stv<T, V>((isq ? qo + (i64)head * a.hd : ko + (i64)(head - a.h) * a.hd) + e0, x);
+        for (int g = 0; g < UNIT; ++g) {
+            if (g >= a.per) break;
+            const int head = head0 + g * HPW;
+            const bool isq = head < a.h;
+            float x[V];
+            unpack<T, V>(raw[g], x);
+            float ss = 0.f;
+#pragma unroll
+            for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
+            const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
+            if (!in || head >= heads) continue;
+#pragma unroll
+            for (int u = 0; u < V; ++u) x[u] = x[u] * r * (isq ? wq[u] : wk[u]);
+            rotate<V>(x, cs);
+            stv<T, V>(isq ? qo + (i64)head * a.hd : ko + (i64)(head - a.h) * a.hd, x);
+        }
     }
 }
 
@@ -178,65 +205,65 @@ struct BwdArgs {
     const float *wq, *wk;
     const int32_t* pos;
     void *dq, *dk;
-    float* part;  // [CTAs][2·hd]: each CTA's sums for wq, then wk
+    float* part;  // a row of hd sums from each CTA: those of wq, then those of wk
     i64 tokens, s;
     int h, hkv, hd;
     float eps;
-    int per, uq, units;  // groups a unit takes; query units and all units of a token
+    int per[2], units[2];  // groups of a unit and units of a token, of queries and of keys
+    int q_ctas;            // CTAs that have the queries; the others have the keys
 };
 
-// Adjoint on 16-byte pieces. A unit holds up to `per` groups of one token,
-// of query heads (units [0, uq)) or of key heads, so that its weight sums go
-// to one accumulator; warps walk the units in grid order and keep both.
+// Adjoint on 16-byte pieces. A CTA has query heads or key heads, so that it
+// holds one weight and one sum; both kinds walk their units in grid order.
+constexpr int BWD_UNIT = 4;
 template <typename T, int LPH>
-__global__ void __launch_bounds__(WARPS * 32) k_qk_bwd(const __grid_constant__ BwdArgs a, const __grid_constant__ Freq f) {
+__global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant__ BwdArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
-    __shared__ float sum[WARPS][2][MAX_HD];
+    __shared__ float sum[WARPS][MAX_HD];
+    tc::launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH, li = lane % LPH, e0 = li * V;
-    const bool in = e0 < a.hd;
-    float wv[2][V], acc[2][V];
+    const bool in = e0 < a.hd, isq = (int)blockIdx.x < a.q_ctas;
+    const int heads = isq ? a.h : a.hkv, per = isq ? a.per[0] : a.per[1], units = isq ? a.units[0] : a.units[1];
+    const i64 xs = isq ? a.q_stride : a.k_stride, gs = isq ? a.gq_stride : a.gk_stride;
+    const T* const xp = (const T*)(isq ? a.q : a.k) + e0;
+    const T* const gp = (const T*)(isq ? a.gq : a.gk) + e0;
+    T* const dp = (T*)(isq ? a.dq : a.dk) + e0;
+    float w[V], acc[V];
 #pragma unroll
-    for (int u = 0; u < V; ++u) wv[0][u] = wv[1][u] = acc[0][u] = acc[1][u] = 0.f;
-    if (in) {
-        ldv<float, V>(a.wq + e0, wv[0]);
-        ldv<float, V>(a.wk + e0, wv[1]);
-    }
-    const i64 all = a.tokens * a.units;
-    for (i64 unit = (i64)blockIdx.x * WARPS + warp; unit < all; unit += (i64)gridDim.x * WARPS) {
-        const i64 tok = unit / a.units;
-        int part = (int)(unit - tok * a.units);
-        const bool isq = part < a.uq;
-        if (!isq) part -= a.uq;
-        const int heads = isq ? a.h : a.hkv, g0 = part * a.per, g1 = min(g0 + a.per, (heads + HPW - 1) / HPW);
-        const T* xrow = isq ? (const T*)a.q + tok * a.q_stride : (const T*)a.k + tok * a.k_stride;
-        const T* grow = isq ? (const T*)a.gq + tok * a.gq_stride : (const T*)a.gk + tok * a.gk_stride;
-        T* drow = (isq ? (T*)a.dq : (T*)a.dk) + tok * heads * a.hd;
+    for (int u = 0; u < V; ++u) w[u] = acc[u] = 0.f;
+    if (in) ldv<float, V>((isq ? a.wq : a.wk) + e0, w);
+    const i64 all = a.tokens * units;
+    const int cta = isq ? blockIdx.x : blockIdx.x - a.q_ctas, ctas = isq ? a.q_ctas : gridDim.x - a.q_ctas;
+    for (i64 unit = (i64)cta * WARPS + warp; unit < all; unit += (i64)ctas * WARPS) {
+        const i64 tok = units == 1 ? unit : unit / units;
+        const int head0 = (int)(unit - tok * units) * per * HPW + sub;
+        uint4 xr[BWD_UNIT], yr[BWD_UNIT];
+#pragma unroll
+        for (int g = 0; g < BWD_UNIT; ++g) {
+            const int head = head0 + g * HPW;
+            xr[g] = yr[g] = make_uint4(0, 0, 0, 0);
+            if (g < per && in && head < heads) {
+                xr[g] = *(const uint4*)(xp + tok * xs + (i64)head * a.hd);
+                yr[g] = *(const uint4*)(gp + tok * gs + (i64)head * a.hd);
+            }
+        }
         const int p = a.pos ? a.pos[tok] : (int)(tok % a.s);
         float2 cs[V / 2];
-        float w[V], dw[V];
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-            w[u] = isq ? wv[0][u] : wv[1][u];
-            dw[u] = 0.f;
-        }
-        if (in) {
+        if (in)
 #pragma unroll
             for (int u = 0; u < V / 2; ++u) {
                 cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
                 cs[u].y = -cs[u].y;
             }
-        }
-        for (int g = g0; g < g1; ++g) {
-            const int head = g * HPW + sub;
+#pragma unroll
+        for (int g = 0; g < BWD_UNIT; ++g) {
+            if (g >= per) break;
+            const int head = head0 + g * HPW;
             const bool on = in && head < heads;
             float x[V], y[V];
-#pragma unroll
-            for (int u = 0; u < V; ++u) x[u] = y[u] = 0.f;
-            if (on) {
-                ldv<T, V>(xrow + (i64)head * a.hd + e0, x);
-                ldv<T, V>(grow + (i64)head * a.hd + e0, y);
-                rotate<V>(y, cs);
-            }
+            unpack<T, V>(xr[g], x);
+            unpack<T, V>(yr[g], y);
+            if (on) rotate<V>(y, cs);
             float ss = 0.f, dot = 0.f;
 #pragma unroll
             for (int u = 0; u < V; ++u) {
@@ -249,40 +276,32 @@ __global__ void __launch_bounds__(WARPS * 32) k_qk_bwd(const __grid_constant__ B
 #pragma unroll
             for (int u = 0; u < V; ++u) {
                 const float xh = x[u] * r;
-                dw[u] = fmaf(y[u], xh, dw[u]);
+                acc[u] = fmaf(y[u], xh, acc[u]);
                 x[u] = r * (y[u] * w[u] - xh * dot);
             }
-            stv<T, V>(drow + (i64)head * a.hd + e0, x);
-        }
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-            acc[0][u] += isq ? dw[u] : 0.f;
-            acc[1][u] += isq ? 0.f : dw[u];
+            stv<T, V>(dp + (tok * heads + head) * a.hd, x);
         }
     }
     // the groups of a warp, then the warps of the CTA, each in a fixed order
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int u = 0; u < V; ++u) {
 #pragma unroll
-        for (int u = 0; u < V; ++u) {
-            float v = acc[m][u];
-#pragma unroll
-            for (int o = 16; o >= LPH; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (sub == 0 && in) sum[warp][m][e0 + u] = v;
-        }
+        for (int o = 16; o >= LPH; o >>= 1) acc[u] += __shfl_xor_sync(0xffffffffu, acc[u], o);
+        if (sub == 0 && in) sum[warp][e0 + u] = acc[u];
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.hd; i += WARPS * 32) {
-        const int m = i >= a.hd, e = i - m * a.hd;
+    for (int e = threadIdx.x; e < a.hd; e += WARPS * 32) {
         float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < WARPS; ++j) v += sum[j][m][e];
-        a.part[(i64)blockIdx.x * 2 * a.hd + i] = v;
+        for (int j = 0; j < WARPS; ++j) v += sum[j][e];
+        a.part[(i64)blockIdx.x * a.hd + e] = v;
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32) k_qk_bwd_any(const __grid_constant__ BwdArgs a, const __grid_constant__ Freq f) {
     __shared__ float sum[WARPS][2][MAX_HD];
+    tc::launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = a.h + a.hkv;
     float acc[2][2 * PAIRS];
 #pragma unroll
@@ -340,29 +359,33 @@ __global__ void __launch_bounds__(WARPS * 32) k_qk_bwd_any(const __grid_constant
         float v = 0.f;
 #pragma unroll
         for (int j = 0; j < WARPS; ++j) v += sum[j][m][e];
-        a.part[(i64)blockIdx.x * 2 * a.hd + i] = v;
+        a.part[((i64)m * gridDim.x + blockIdx.x) * a.hd + e] = v;
     }
 }
 
 // dw = the CTAs' sums added up in a fixed order: 8 columns a CTA, 32 row
 // groups of which each adds every 32nd row, then the groups in order.
+// Columns [0, hd) are wq's, over rows [0, rows_q); the rest wk's, over the
+// rows_k rows behind them.
 constexpr int FIN_COLS = 8, FIN_ROWS = 32;
-__global__ void __launch_bounds__(FIN_COLS * FIN_ROWS) k_qk_dw(const float* __restrict__ part, int rows, int hd,
+__global__ void __launch_bounds__(FIN_COLS * FIN_ROWS) k_qk_dw(const float* __restrict__ part, int rows_q, int rows_k, int hd,
                                                               float* __restrict__ dwq, float* __restrict__ dwk) {
     __shared__ float s[FIN_ROWS][FIN_COLS];
     const int cx = threadIdx.x % FIN_COLS, ry = threadIdx.x / FIN_COLS, col = blockIdx.x * FIN_COLS + cx;
+    const bool isq = col < hd;
+    const int e = isq ? col : col - hd, r0 = isq ? 0 : rows_q, rows = isq ? rows_q : rows_k;
+    tc::grid_dependency_wait();
     float v = 0.f;
     if (col < 2 * hd)
 #pragma unroll 8
-        for (int r = ry; r < rows; r += FIN_ROWS) v += part[(i64)r * 2 * hd + col];
+        for (int r = ry; r < rows; r += FIN_ROWS) v += __ldcg(part + (i64)(r0 + r) * hd + e);
     s[ry][cx] = v;
     __syncthreads();
     if (ry == 0 && col < 2 * hd) {
         v = 0.f;
 #pragma unroll
         for (int r = 0; r < FIN_ROWS; ++r) v += s[r][cx];
-        if (col < hd) dwq[col] = v;
-        else dwk[col - hd] = v;
+        (isq ? dwq : dwk)[e] = v;
     }
 }
 
@@ -390,56 +413,64 @@ __device__ __forceinline__ i64 cache_row(const AppendArgs& a, i64 seq, int pos) 
 
 // Rows of a token: H query heads to qo, Hkv key heads and Hkv value heads to
 // their slot. Query rows of a token that belongs to no sequence become zero.
+// The rows are on their way before the token's place is looked up.
 template <typename T, int LPH>
-__global__ void __launch_bounds__(WARPS * 32) k_append(const __grid_constant__ AppendArgs a, const __grid_constant__ Freq f) {
+__global__ void __launch_bounds__(WARPS * 32, 3) k_append(const __grid_constant__ AppendArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
-    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V;
-    const i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const i64 tok = unit / a.units;
-    if (tok >= a.tokens) return;
-    const int rows = a.h + 2 * a.hkv, g0 = (int)(unit - tok * a.units) * a.per, g1 = min(g0 + a.per, (rows + HPW - 1) / HPW);
+    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V, rows = a.h + 2 * a.hkv;
     const bool in = e0 < a.hd, norm = a.wq != nullptr;
-    i64 seq = 0;
-    const int p = place::token_position(a.lens, a.cu, a.seqs, tok, seq);
-    const i64 base = p >= 0 ? cache_row(a, seq, p) : -1;
     float wq[V], wk[V];
-    float2 cs[V / 2];
 #pragma unroll
     for (int u = 0; u < V; ++u) wq[u] = wk[u] = 1.f;
-    if (in) {
-        if (norm) {
-            ldv<float, V>(a.wq + e0, wq);
-            ldv<float, V>(a.wk + e0, wk);
-        }
-#pragma unroll
-        for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
+    if (in && norm) {
+        ldv<float, V>(a.wq + e0, wq);
+        ldv<float, V>(a.wk + e0, wk);
     }
-    const T* qrow = (const T*)a.q + tok * a.q_stride;
-    const T* krow = (const T*)a.k + tok * a.k_stride;
-    const T* vrow = (const T*)a.v + tok * a.v_stride;
-    for (int g = g0; g < g1; ++g) {
-        const int row = g * HPW + sub;
-        const bool on = in && row < rows;
-        const int kind = row < a.h ? 0 : row < a.h + a.hkv ? 1 : 2, head = kind == 0 ? row : kind == 1 ? row - a.h : row - a.h - a.hkv;
-        float x[V];
+    const i64 all = a.tokens * a.units;
+    for (i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += (i64)gridDim.x * WARPS) {
+        const i64 tok = a.units == 1 ? unit : unit / a.units;
+        const int row0 = (int)(unit - tok * a.units) * a.per * HPW + sub;
+        const T* qrow = (const T*)a.q + tok * a.q_stride + e0;
+        const T* krow = (const T*)a.k + tok * a.k_stride + e0;
+        const T* vrow = (const T*)a.v + tok * a.v_stride + e0;
+        uint4 raw[UNIT];
 #pragma unroll
-        for (int u = 0; u < V; ++u) x[u] = 0.f;
-        if (on && p >= 0) ldv<T, V>((kind == 0 ? qrow : kind == 1 ? krow : vrow) + (i64)head * a.hd + e0, x);
-        float r = 1.f;
-        if (norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
-            r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
+        for (int g = 0; g < UNIT; ++g) {
+            const int row = row0 + g * HPW, kr = row - a.h, vr = kr - a.hkv;
+            raw[g] = make_uint4(0, 0, 0, 0);
+            if (g < a.per && in && row < rows)
+                raw[g] = *(const uint4*)(kr < 0 ? qrow + (i64)row * a.hd : vr < 0 ? krow + (i64)kr * a.hd : vrow + (i64)vr * a.hd);
         }
-        if (!on) continue;
-        if (kind < 2 && p >= 0) {
+        i64 seq = 0;
+        const int p = place::token_position(a.lens, a.cu, a.seqs, tok, seq);
+        const i64 base = p >= 0 ? cache_row(a, seq, p) : -1;
+        float2 cs[V / 2];
+        if (in)
 #pragma unroll
-            for (int u = 0; u < V; ++u) x[u] = x[u] * r * (kind == 0 ? wq[u] : wk[u]);
-            rotate<V>(x, cs);
+            for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
+        T* qo = (T*)a.qo + tok * a.h * a.hd + e0;
+#pragma unroll
+        for (int g = 0; g < UNIT; ++g) {
+            if (g >= a.per) break;
+            const int row = row0 + g * HPW, kr = row - a.h, vr = kr - a.hkv;
+            const bool on = in && row < rows;
+            float r = 1.f, x[V];
+            unpack<T, V>(raw[g], x);
+            if (norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
+                r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
+            }
+            if (!on) continue;
+            if (vr < 0) {
+#pragma unroll
+                for (int u = 0; u < V; ++u) x[u] = p >= 0 ? x[u] * r * (kr < 0 ? wq[u] : wk[u]) : 0.f;
+                rotate<V>(x, cs);
+            }
+            if (kr < 0) stv<T, V>(qo + (i64)row * a.hd, x);
+            else if (base >= 0) stv<T, V>((T*)(vr < 0 ? a.kc : a.vc) + base + (i64)(vr < 0 ? kr : vr) * a.page * a.hd + e0, x);
         }
-        if (kind == 0) stv<T, V>((T*)a.qo + (tok * a.h + head) * a.hd + e0, x);
-        else if (base >= 0) stv<T, V>((T*)(kind == 1 ? a.kc : a.vc) + base + (i64)head * a.page * a.hd + e0, x);
     }
 }
 
@@ -492,12 +523,12 @@ __global__ void __launch_bounds__(WARPS * 32) k_append_any(const __grid_constant
 }
 
 // ------------------------------------------------------------ launchers
-// Groups of HPW rows that a warp takes of one token: all of them (the sines
-// are then taken once a token), unless that would leave SMs without warps.
-static int groups_per_warp(Context* c, i64 tokens, int groups) {
-    const i64 want = (i64)c->sm_count * 32;
-    i64 per = tokens * groups / want;
-    return (int)std::max<i64>(1, std::min<i64>(groups, per));
+// Groups of HPW rows that a unit takes of one token: as many as fit (the
+// sines are then taken once a token), unless that would leave SMs without warps.
+static int groups_per_unit(Context* c, i64 tokens, int groups, int most) {
+    const i64 want = (i64)c->sm_count * 16;
+    const int units = cdiv(groups, (int)std::max<i64>(1, std::min<i64>(most, tokens * groups / want)));
+    return cdiv(groups, units);
 }
 
 static int lanes_of(int hd, int vec) {
@@ -546,9 +577,9 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && aligned_to(qo, 16) &&
         aligned_to(ko, 16) && aligned_to(wq, 16) && aligned_to(wk, 16)) {
         const int groups = cdiv(h + hkv, 32 / lph);
-        a.per = groups_per_warp(c, tokens, groups);
+        a.per = groups_per_unit(c, tokens, groups, UNIT);
         a.units = cdiv(groups, a.per);
-        const int grid = grid_of(tokens * a.units, "qk_norm_rope");
+        const int grid = (int)std::min<i64>((tokens * a.units + WARPS - 1) / WARPS, c->sm_count * 3);
 #define RUN(T, L) k_qk_fwd<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
@@ -561,11 +592,12 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
 }
 
 // CTAs of the adjoint: what the SMs hold at once, each walking many tokens,
-// because every CTA adds one row to the weight sums.
-static i64 qk_bwd_ctas(Context* c, i64 rows) { return std::min<i64>((i64)c->sm_count * 4, (rows + WARPS - 1) / WARPS); }
+// because every CTA adds a row to the weight sums.
+static i64 qk_bwd_ctas(Context* c, i64 rows) { return std::min<i64>((i64)c->sm_count * 2, (rows + WARPS - 1) / WARPS); }
 
+// At least one CTA each for queries and keys, two rows a CTA where it has both.
 size_t qk_norm_rope_bwd_workspace(Context* c, i64 b, i64 s, i64 h, i64 hkv, i64 hd) {
-    return (size_t)qk_bwd_ctas(c, b * s * (h + hkv)) * 2 * hd * sizeof(float);
+    return (size_t)(qk_bwd_ctas(c, b * s * (h + hkv)) + 1) * 2 * hd * sizeof(float);
 }
 
 void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const float* wq, const float* wk,
@@ -576,29 +608,44 @@ void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     check_heads(tokens, h, hkv, hd, "qk_norm_rope backward");
     const Freq& f = freq_of(c, hd, theta);
     BwdArgs a{q, k, gq, gk, q_stride, k_stride, gq_stride, gk_stride, wq, wk, pos, dq, dk, work, tokens, s, (int)h, (int)hkv,
-              (int)hd, eps, 1, 1, 1};
-    int ctas = 0;
+              (int)hd, eps, {1, 1}, {1, 1}, 0};
+    int rows_q = 0, rows_k = 0;
     if (tokens > 0) {
         const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
         if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && rows_ok(gq, gq_stride, hd, vec) &&
             rows_ok(gk, gk_stride, hd, vec) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(wq, 16) &&
             aligned_to(wk, 16)) {
-            const int gh = cdiv(h, 32 / lph), gk_ = cdiv(hkv, 32 / lph);
-            a.per = groups_per_warp(c, tokens, std::max(gh, gk_));
-            a.uq = cdiv(gh, a.per);
-            a.units = a.uq + cdiv(gk_, a.per);
-            ctas = (int)qk_bwd_ctas(c, tokens * a.units);
-#define RUN(T, L) k_qk_bwd<T, L><<<ctas, WARPS * 32, 0, c->stream>>>(a, f)
+            const int groups[2] = {cdiv(h, 32 / lph), cdiv(hkv, 32 / lph)};
+            for (int m = 0; m < 2; ++m) {
+                a.per[m] = groups_per_unit(c, tokens, groups[m], BWD_UNIT);
+                a.units[m] = cdiv(groups[m], a.per[m]);
+            }
+            // CTAs in the proportion of the row groups, none without a unit
+            const i64 uq = tokens * a.units[0], uk = tokens * a.units[1], ctas = std::max<i64>(2, qk_bwd_ctas(c, uq + uk));
+            const i64 share = ctas * groups[0] / (groups[0] + groups[1]);
+            rows_q = (int)std::min<i64>(std::max<i64>(1, std::min(share, ctas - 1)), (uq + WARPS - 1) / WARPS);
+            rows_k = (int)std::min<i64>(ctas - rows_q, (uk + WARPS - 1) / WARPS);
+            a.q_ctas = rows_q;
+#define RUN(T, L) k_qk_bwd<T, L><<<rows_q + rows_k, WARPS * 32, 0, c->stream>>>(a, f)
             if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
         } else {
-            ctas = (int)qk_bwd_ctas(c, tokens * (h + hkv));
-            if (dtype == CATNN_BF16) k_qk_bwd_any<bf16><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
-            else k_qk_bwd_any<float><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
+            rows_q = rows_k = (int)qk_bwd_ctas(c, tokens * (h + hkv));
+            if (dtype == CATNN_BF16) k_qk_bwd_any<bf16><<<rows_q, WARPS * 32, 0, c->stream>>>(a, f);
+            else k_qk_bwd_any<float><<<rows_q, WARPS * 32, 0, c->stream>>>(a, f);
         }
         launched(c);
     }
-    k_qk_dw<<<cdiv(2 * hd, FIN_COLS), FIN_COLS * FIN_ROWS, 0, c->stream>>>(work, ctas, (int)hd, dwq, dwk);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cdiv(2 * hd, FIN_COLS));
+    cfg.blockDim = dim3(FIN_COLS * FIN_ROWS);
+    cfg.stream = c->stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = tokens > 0 ? 1 : 0;  // with no tokens there is no first kernel that lets this one start
+    CUDA_OK(cudaLaunchKernelEx(&cfg, k_qk_dw, (const float*)work, rows_q, rows_k, (int)hd, dwq, dwk));
     launched(c);
 }
 
@@ -615,9 +662,9 @@ void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_str
     if (lph <= 32 && (!q || rows_ok(q, q_stride, hd, vec)) && rows_ok(k, k_stride, hd, vec) && rows_ok(v, v_stride, hd, vec) &&
         aligned_to(qo, 16) && aligned_to(kc, 16) && aligned_to(vc, 16) && aligned_to(wq, 16) && aligned_to(wk, 16)) {
         const int groups = cdiv(h + 2 * hkv, 32 / lph);
-        a.per = groups_per_warp(c, tokens, groups);
+        a.per = groups_per_unit(c, tokens, groups, UNIT);
         a.units = cdiv(groups, a.per);
-        const int grid = grid_of(tokens * a.units, "kv_append");
+        const int grid = (int)std::min<i64>((tokens * a.units + WARPS - 1) / WARPS, c->sm_count * 3);
 #define RUN(T, L) k_append<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN

@@ -66,13 +66,132 @@ template <int LPH> __device__ __forceinline__ float group_sum(float v) {
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 
-template <int V> __device__ __forceinline__ void rotate(float (&x)[V], const float2 (&cs)[V / 2]) {
-#pragma unroll
-    for (int u = 0; u < V / 2; ++u) {
-        float a = x[2 * u], b = x[2 * u + 1];
-        x[2 * u] = a * cs[u].x - b * cs[u].y;
-        x[2 * u + 1] = a * cs[u].y + b * cs[u].x;
+// Two floats in one register pair, for the instructions that work on both.
+// What bounds these kernels next to HBM is the number of instructions, so a
+// lane's values are taken two pairs at a time: X0 = the first elements of
+// pairs i and i + 1, X1 = their second elements.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split2(f2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+    const float2 s = split2(v);
+    return s.x + s.y;
+}
+
+// 16 bytes as packed pairs, and back.
+template <typename T> constexpr int NP = VEC<T> / 4;
+template <typename T> __device__ __forceinline__ void unpack(const uint4& r, f2 (&x0)[NP<T>], f2 (&x1)[NP<T>]) {
+    if constexpr (sizeof(T) == 4) {
+        x0[0] = pack2(__uint_as_float(r.x), __uint_as_float(r.z));
+        x1[0] = pack2(__uint_as_float(r.y), __uint_as_float(r.w));
+    } else {
+        x0[0] = pack2(__uint_as_float(r.x << 16), __uint_as_float(r.y << 16));
+        x1[0] = pack2(__uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y & 0xffff0000u));
+        x0[1] = pack2(__uint_as_float(r.z << 16), __uint_as_float(r.w << 16));
+        x1[1] = pack2(__uint_as_float(r.z & 0xffff0000u), __uint_as_float(r.w & 0xffff0000u));
     }
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+template <typename T> __device__ __forceinline__ uint4 repack(const f2 (&x0)[NP<T>], const f2 (&x1)[NP<T>]) {
+    const float2 a = split2(x0[0]), b = split2(x1[0]);
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(a.x), __float_as_uint(b.x), __float_as_uint(a.y), __float_as_uint(b.y));
+    } else {
+        const float2 c = split2(x0[1]), d = split2(x1[1]);
+        return make_uint4(bf16x2(a.x, b.x), bf16x2(a.y, b.y), bf16x2(c.x, d.x), bf16x2(c.y, d.y));
+    }
+}
+
+// A lane's cosines and sines at a position.
+template <typename T> struct Turn {
+    f2 c[NP<T>], s[NP<T>];
+    __device__ __forceinline__ void at(int pos, const Freq& f, int pair0) {
+#pragma unroll
+        for (int j = 0; j < NP<T>; ++j) {
+            const float2 a = cos_sin<T>(pos, f.turn[pair0 + 2 * j]), b = cos_sin<T>(pos, f.turn[pair0 + 2 * j + 1]);
+            c[j] = pack2(a.x, b.x);
+            s[j] = pack2(a.y, b.y);
+        }
+    }
+};
+// The norm's weights of a lane's pairs, out of shared memory.
+template <typename T> __device__ __forceinline__ void weights(const float* w, f2 (&w0)[NP<T>], f2 (&w1)[NP<T>]) {
+#pragma unroll
+    for (int j = 0; j < NP<T>; ++j) {
+        const float4 v = *(const float4*)(w + 4 * j);
+        w0[j] = pack2(v.x, v.z);
+        w1[j] = pack2(v.y, v.w);
+    }
+}
+// Weight and rotation in one: y0 = x0·a + x1·b, y1 = x0·c + x1·d.
+template <typename T> struct Coef {
+    f2 a[NP<T>], b[NP<T>], c[NP<T>], d[NP<T>];
+    __device__ __forceinline__ void of(const Turn<T>& t, const float* w) {
+        f2 w0[NP<T>], w1[NP<T>];
+        weights<T>(w, w0, w1);
+        const f2 minus = pack2(-1.f, -1.f);
+#pragma unroll
+        for (int j = 0; j < NP<T>; ++j) {
+            a[j] = mul2(w0[j], t.c[j]);
+            b[j] = mul2(mul2(w1[j], t.s[j]), minus);
+            c[j] = mul2(w0[j], t.s[j]);
+            d[j] = mul2(w1[j], t.c[j]);
+        }
+    }
+};
+
+// One row: its norm (where `norm`), weights and rotation.
+template <typename T, int LPH>
+__device__ __forceinline__ uint4 norm_turn(const uint4& raw, const Coef<T>& k, bool norm, float inv_hd, float eps) {
+    f2 x0[NP<T>], x1[NP<T>], y0[NP<T>], y1[NP<T>];
+    unpack<T>(raw, x0, x1);
+    f2 r = pack2(1.f, 1.f);
+    if (norm) {
+        f2 ss = mul2(x0[0], x0[0]);
+        ss = fma2(x1[0], x1[0], ss);
+        if (NP<T> > 1) {
+            ss = fma2(x0[NP<T> - 1], x0[NP<T> - 1], ss);
+            ss = fma2(x1[NP<T> - 1], x1[NP<T> - 1], ss);
+        }
+        const float v = rsqrtf(fmaf(group_sum<LPH>(sum2(ss)), inv_hd, eps));
+        r = pack2(v, v);
+    }
+#pragma unroll
+    for (int j = 0; j < NP<T>; ++j) {
+        y0[j] = mul2(fma2(x1[j], k.b[j], mul2(x0[j], k.a[j])), r);
+        y1[j] = mul2(fma2(x1[j], k.d[j], mul2(x0[j], k.c[j])), r);
+    }
+    return repack<T>(y0, y1);
+}
+
+// The weights in shared memory, once a CTA; 1 where there are none.
+__device__ __forceinline__ void load_weights(float (&sw)[2][MAX_HD], const float* wq, const float* wk, int hd) {
+    for (int i = threadIdx.x; i < MAX_HD; i += blockDim.x) {
+        sw[0][i] = i < hd && wq ? wq[i] : 1.f;
+        sw[1][i] = i < hd && wk ? wk[i] : 1.f;
+    }
+    __syncthreads();
 }
 
 struct FwdArgs {
@@ -83,79 +202,48 @@ struct FwdArgs {
     void *qo, *ko;
     i64 tokens, s;
     int h, hkv, hd;
-    float eps;
-    // a unit is up to `per` row groups of a token, `units` units a token
-    int per, units;
+    float eps, inv_hd;
+    // row groups of a token: gq of its query heads, then those of its key
+    // heads; a unit is `per` of them, `units` units a token
+    int gq, per, units;
 };
 
-// 16 bytes as V values.
-template <typename T, int V> __device__ __forceinline__ void unpack(const uint4& r, float (&o)[V]) {
-    if constexpr (sizeof(T) == 4) {
-        o[0] = __uint_as_float(r.x), o[1] = __uint_as_float(r.y), o[2] = __uint_as_float(r.z), o[3] = __uint_as_float(r.w);
-    } else {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[2 * j] = __uint_as_float(w[j] << 16);
-            o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    }
-}
-
-// Forward on 16-byte pieces. Group g of a token holds heads
-// [g·HPW, (g+1)·HPW) of its H query heads followed by its Hkv key heads. A
-// warp walks the units in grid order; all rows of a unit are on their way
-// before its sines are taken.
+// Forward on 16-byte pieces. A group is the HPW = 32 / LPH heads that a warp
+// takes at once. A warp walks the units in grid order; all rows of a unit are
+// on their way before its sines are taken.
 constexpr int UNIT = 6;  // row groups of a unit, at most
 template <typename T, int LPH>
 __global__ void __launch_bounds__(WARPS * 32, 3) k_qk_fwd(const __grid_constant__ FwdArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
-    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V, heads = a.h + a.hkv;
+    __shared__ __align__(16) float sw[2][MAX_HD];
+    const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd;
-    float wq[V], wk[V];
-#pragma unroll
-    for (int u = 0; u < V; ++u) wq[u] = wk[u] = 0.f;
-    if (in) {
-        ldv<float, V>(a.wq + e0, wq);
-        ldv<float, V>(a.wk + e0, wk);
-    }
-    const i64 all = a.tokens * a.units;
-    for (i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += (i64)gridDim.x * WARPS) {
-        const i64 tok = a.units == 1 ? unit : unit / a.units;
-        const int head0 = (int)(unit - tok * a.units) * a.per * HPW + sub;
-        const T* qrow = (const T*)a.q + tok * a.q_stride + e0;
-        const T* krow = (const T*)a.k + tok * a.k_stride + e0;
+    load_weights(sw, a.wq, a.wk, a.hd);
+    const int all = (int)a.tokens * a.units;
+    for (int unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += gridDim.x * WARPS) {
+        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per, nq = a.gq - g0;
+        // group g is a query group for g < nq
+        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+        const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
+        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;  // group g is there for g·HPW below
         uint4 raw[UNIT];
 #pragma unroll
         for (int g = 0; g < UNIT; ++g) {
-            const int head = head0 + g * HPW;
             raw[g] = make_uint4(0, 0, 0, 0);
-            if (g < a.per && in && head < heads)
-                raw[g] = *(const uint4*)(head < a.h ? qrow + (i64)head * a.hd : krow + (i64)(head - a.h) * a.hd);
+            if (g < a.per && g * HPW < (g < nq ? hq : hk)) raw[g] = *(const uint4*)((g < nq ? q : k) + g * step);
         }
-        const int p = a.pos ? a.pos[tok] : (int)(tok % a.s);
-        float2 cs[V / 2];
-        if (in)
-#pragma unroll
-            for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
-        T* qo = (T*)a.qo + tok * a.h * a.hd + e0;
-        T* ko = (T*)a.ko + tok * a.hkv * a.hd + e0;
+        Turn<T> t;
+        t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
+        T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
+        T* const ko = (T*)a.ko + (i64)tok * a.hkv * a.hd + off - nq * step;
+        Coef<T> c;
+        if (nq > 0) c.of(t, sw[0] + e0);
 #pragma unroll
         for (int g = 0; g < UNIT; ++g) {
             if (g >= a.per) break;
-            const int head = head0 + g * HPW;
-            const bool isq = head < a.h;
-            float x[V];
-            unpack<T, V>(raw[g], x);
-            float ss = 0.f;
-#pragma unroll
-            for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
-            const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
-            if (!in || head >= heads) continue;
-#pragma unroll
-            for (int u = 0; u < V; ++u) x[u] = x[u] * r * (isq ? wq[u] : wk[u]);
-            rotate<V>(x, cs);
-            stv<T, V>(isq ? qo + (i64)head * a.hd : ko + (i64)(head - a.h) * a.hd, x);
+            if (g == max(nq, 0)) c.of(t, sw[1] + e0);
+            const uint4 y = norm_turn<T, LPH>(raw[g], c, true, a.inv_hd, a.eps);
+            if (g * HPW < (g < nq ? hq : hk)) *(uint4*)((g < nq ? qo : ko) + g * step) = y;
         }
     }
 }
@@ -205,96 +293,120 @@ struct BwdArgs {
     const float *wq, *wk;
     const int32_t* pos;
     void *dq, *dk;
-    float* part;  // a row of hd sums from each CTA: those of wq, then those of wk
+    float* part;  // [2][CTAs][hd]: each CTA's sums for wq, then for wk
     i64 tokens, s;
     int h, hkv, hd;
-    float eps;
-    int per[2], units[2];  // groups of a unit and units of a token, of queries and of keys
-    int q_ctas;            // CTAs that have the queries; the others have the keys
+    float eps, inv_hd;
+    int groups_q, per, units;  // as in the forward
 };
 
-// Adjoint on 16-byte pieces. A CTA has query heads or key heads, so that it
-// holds one weight and one sum; both kinds walk their units in grid order.
-constexpr int BWD_UNIT = 4;
+// Adjoint on 16-byte pieces, units as in the forward; both weight sums stay in
+// registers over all units of a warp.
+constexpr int BWD_UNIT = 5;
 template <typename T, int LPH>
 __global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant__ BwdArgs a, const __grid_constant__ Freq f) {
-    constexpr int V = VEC<T>, HPW = 32 / LPH;
+    constexpr int V = VEC<T>, N = NP<T>, HPW = 32 / LPH;
+    __shared__ __align__(16) float sw[2][MAX_HD];
     __shared__ float sum[WARPS][MAX_HD];
     tc::launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH, li = lane % LPH, e0 = li * V;
-    const bool in = e0 < a.hd, isq = (int)blockIdx.x < a.q_ctas;
-    const int heads = isq ? a.h : a.hkv, per = isq ? a.per[0] : a.per[1], units = isq ? a.units[0] : a.units[1];
-    const i64 xs = isq ? a.q_stride : a.k_stride, gs = isq ? a.gq_stride : a.gk_stride;
-    const T* const xp = (const T*)(isq ? a.q : a.k) + e0;
-    const T* const gp = (const T*)(isq ? a.gq : a.gk) + e0;
-    T* const dp = (T*)(isq ? a.dq : a.dk) + e0;
-    float w[V], acc[V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd;
+    const int off = sub * a.hd + e0;
+    const bool in = e0 < a.hd;
+    load_weights(sw, a.wq, a.wk, a.hd);
+    f2 acc[2][2][N];  // of queries and keys, of first and second elements
 #pragma unroll
-    for (int u = 0; u < V; ++u) w[u] = acc[u] = 0.f;
-    if (in) ldv<float, V>((isq ? a.wq : a.wk) + e0, w);
-    const i64 all = a.tokens * units;
-    const int cta = isq ? blockIdx.x : blockIdx.x - a.q_ctas, ctas = isq ? a.q_ctas : gridDim.x - a.q_ctas;
-    for (i64 unit = (i64)cta * WARPS + warp; unit < all; unit += (i64)ctas * WARPS) {
-        const i64 tok = units == 1 ? unit : unit / units;
-        const int head0 = (int)(unit - tok * units) * per * HPW + sub;
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[m][0][j] = acc[m][1][j] = pack2(0.f, 0.f);
+    const int all = (int)a.tokens * a.units;
+    for (int unit = blockIdx.x * WARPS + warp; unit < all; unit += gridDim.x * WARPS) {
+        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per, nq = a.groups_q - g0;
+        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+        const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
+        const T* const gq = (const T*)a.gq + tok * a.gq_stride + off + g0 * step;
+        const T* const gk = (const T*)a.gk + tok * a.gk_stride + off - nq * step;
+        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;
         uint4 xr[BWD_UNIT], yr[BWD_UNIT];
 #pragma unroll
         for (int g = 0; g < BWD_UNIT; ++g) {
-            const int head = head0 + g * HPW;
             xr[g] = yr[g] = make_uint4(0, 0, 0, 0);
-            if (g < per && in && head < heads) {
-                xr[g] = *(const uint4*)(xp + tok * xs + (i64)head * a.hd);
-                yr[g] = *(const uint4*)(gp + tok * gs + (i64)head * a.hd);
+            if (g < a.per && g * HPW < (g < nq ? hq : hk)) {
+                xr[g] = *(const uint4*)((g < nq ? q : k) + g * step);
+                yr[g] = *(const uint4*)((g < nq ? gq : gk) + g * step);
             }
         }
-        const int p = a.pos ? a.pos[tok] : (int)(tok % a.s);
-        float2 cs[V / 2];
-        if (in)
+        Turn<T> t;
+        t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
+        T* const dq = (T*)a.dq + (i64)tok * a.h * a.hd + off + g0 * step;
+        T* const dk = (T*)a.dk + (i64)tok * a.hkv * a.hd + off - nq * step;
+        const f2 minus = pack2(-1.f, -1.f);
+        f2 ns[N], w0[N], w1[N];
 #pragma unroll
-            for (int u = 0; u < V / 2; ++u) {
-                cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
-                cs[u].y = -cs[u].y;
-            }
+        for (int j = 0; j < N; ++j) ns[j] = mul2(t.s[j], minus);
+        weights<T>(sw[nq > 0 ? 0 : 1] + e0, w0, w1);
 #pragma unroll
         for (int g = 0; g < BWD_UNIT; ++g) {
-            if (g >= per) break;
-            const int head = head0 + g * HPW;
-            const bool on = in && head < heads;
-            float x[V], y[V];
-            unpack<T, V>(xr[g], x);
-            unpack<T, V>(yr[g], y);
-            if (on) rotate<V>(y, cs);
-            float ss = 0.f, dot = 0.f;
+            if (g >= a.per) break;
+            if (g > 0 && g == nq) weights<T>(sw[1] + e0, w0, w1);
+            f2 x0[N], x1[N], y0[N], y1[N], g0_[N], g1_[N];
+            unpack<T>(xr[g], x0, x1);
+            unpack<T>(yr[g], y0, y1);
+            f2 ss = pack2(0.f, 0.f), dt = ss;
 #pragma unroll
-            for (int u = 0; u < V; ++u) {
-                ss = fmaf(x[u], x[u], ss);
-                dot = fmaf(y[u] * w[u], x[u], dot);
+            for (int j = 0; j < N; ++j) {
+                g0_[j] = fma2(y1[j], t.s[j], mul2(y0[j], t.c[j]));  // turned back
+                g1_[j] = fma2(y0[j], ns[j], mul2(y1[j], t.c[j]));
+                ss = fma2(x0[j], x0[j], ss);
+                ss = fma2(x1[j], x1[j], ss);
+                y0[j] = mul2(g0_[j], w0[j]);
+                y1[j] = mul2(g1_[j], w1[j]);
+                dt = fma2(y0[j], x0[j], dt);
+                dt = fma2(y1[j], x1[j], dt);
             }
-            const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
-            dot = group_sum<LPH>(dot) * r / (float)a.hd;
-            if (!on) continue;
+            const bool on = g * HPW < (g < nq ? hq : hk);
+            const float mean = fmaf(group_sum<LPH>(sum2(ss)), a.inv_hd, a.eps), r = on ? rsqrtf(mean) : 0.f;
+            const float m = -(group_sum<LPH>(sum2(dt)) * r * a.inv_hd) * r;  // -r·mean(g·w·x̂)
+            const f2 rr = pack2(r, r), mm = pack2(m, m);
 #pragma unroll
-            for (int u = 0; u < V; ++u) {
-                const float xh = x[u] * r;
-                acc[u] = fmaf(y[u], xh, acc[u]);
-                x[u] = r * (y[u] * w[u] - xh * dot);
+            for (int j = 0; j < N; ++j) {
+                x0[j] = mul2(x0[j], rr);
+                x1[j] = mul2(x1[j], rr);
+                // a row that is not there has x = 0 and r = 0 and adds nothing
+                if (g < nq) {
+                    acc[0][0][j] = fma2(g0_[j], x0[j], acc[0][0][j]);
+                    acc[0][1][j] = fma2(g1_[j], x1[j], acc[0][1][j]);
+                } else {
+                    acc[1][0][j] = fma2(g0_[j], x0[j], acc[1][0][j]);
+                    acc[1][1][j] = fma2(g1_[j], x1[j], acc[1][1][j]);
+                }
+                y0[j] = fma2(x0[j], mm, mul2(y0[j], rr));
+                y1[j] = fma2(x1[j], mm, mul2(y1[j], rr));
             }
-            stv<T, V>(dp + (tok * heads + head) * a.hd, x);
+            if (on) *(uint4*)((g < nq ? dq : dk) + g * step) = repack<T>(y0, y1);
         }
     }
     // the groups of a warp, then the warps of the CTA, each in a fixed order
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
+    for (int m = 0; m < 2; ++m) {
 #pragma unroll
-        for (int o = 16; o >= LPH; o >>= 1) acc[u] += __shfl_xor_sync(0xffffffffu, acc[u], o);
-        if (sub == 0 && in) sum[warp][e0 + u] = acc[u];
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.hd; e += WARPS * 32) {
-        float v = 0.f;
+        for (int j = 0; j < N; ++j) {
+            const float2 v0 = split2(acc[m][0][j]), v1 = split2(acc[m][1][j]);
+            float v[4] = {v0.x, v1.x, v0.y, v1.y};
 #pragma unroll
-        for (int j = 0; j < WARPS; ++j) v += sum[j][e];
-        a.part[(i64)blockIdx.x * a.hd + e] = v;
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int o = 16; o >= LPH; o >>= 1) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
+                if (sub == 0 && in) sum[warp][e0 + 4 * j + u] = v[u];
+            }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < a.hd; e += WARPS * 32) {
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < WARPS; ++j) v += sum[j][e];
+            a.part[((i64)m * gridDim.x + blockIdx.x) * a.hd + e] = v;
+        }
+        __syncthreads();
     }
 }
 
@@ -365,15 +477,14 @@ __global__ void __launch_bounds__(WARPS * 32) k_qk_bwd_any(const __grid_constant
 
 // dw = the CTAs' sums added up in a fixed order: 8 columns a CTA, 32 row
 // groups of which each adds every 32nd row, then the groups in order.
-// Columns [0, hd) are wq's, over rows [0, rows_q); the rest wk's, over the
-// rows_k rows behind them.
+// Columns [0, hd) are wq's, the rest wk's, whose rows lie behind wq's.
 constexpr int FIN_COLS = 8, FIN_ROWS = 32;
-__global__ void __launch_bounds__(FIN_COLS * FIN_ROWS) k_qk_dw(const float* __restrict__ part, int rows_q, int rows_k, int hd,
+__global__ void __launch_bounds__(FIN_COLS * FIN_ROWS) k_qk_dw(const float* __restrict__ part, int rows, int hd,
                                                               float* __restrict__ dwq, float* __restrict__ dwk) {
     __shared__ float s[FIN_ROWS][FIN_COLS];
     const int cx = threadIdx.x % FIN_COLS, ry = threadIdx.x / FIN_COLS, col = blockIdx.x * FIN_COLS + cx;
     const bool isq = col < hd;
-    const int e = isq ? col : col - hd, r0 = isq ? 0 : rows_q, rows = isq ? rows_q : rows_k;
+    const int e = isq ? col : col - hd, r0 = isq ? 0 : rows;
     tc::grid_dependency_wait();
     float v = 0.f;
     if (col < 2 * hd)
@@ -399,8 +510,8 @@ struct AppendArgs {
     i64 tokens, seqs;
     int h, hkv, hd, page, max_pages;
     i64 pages;
-    float eps;
-    int per, units;
+    float eps, inv_hd;
+    int gq, gk, per, units;
     int* err;
 };
 
@@ -411,65 +522,53 @@ __device__ __forceinline__ i64 cache_row(const AppendArgs& a, i64 seq, int pos) 
     return at;
 }
 
-// Rows of a token: H query heads to qo, Hkv key heads and Hkv value heads to
-// their slot. Query rows of a token that belongs to no sequence become zero.
-// The rows are on their way before the token's place is looked up.
+// Row groups of a token: gq of its H query heads, which go to qo, then gk of
+// its key heads and as many of its value heads, which go to their slots; the
+// values are copied as they are. Query rows of a token that belongs to no
+// sequence become zero. The rows are on their way before the token's place is
+// looked up.
 template <typename T, int LPH>
 __global__ void __launch_bounds__(WARPS * 32, 3) k_append(const __grid_constant__ AppendArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
-    const int lane = threadIdx.x & 31, sub = lane / LPH, li = lane % LPH, e0 = li * V, rows = a.h + 2 * a.hkv;
+    __shared__ __align__(16) float sw[2][MAX_HD];
+    const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd, norm = a.wq != nullptr;
-    float wq[V], wk[V];
-#pragma unroll
-    for (int u = 0; u < V; ++u) wq[u] = wk[u] = 1.f;
-    if (in && norm) {
-        ldv<float, V>(a.wq + e0, wq);
-        ldv<float, V>(a.wk + e0, wk);
-    }
-    const i64 all = a.tokens * a.units;
-    for (i64 unit = (i64)blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += (i64)gridDim.x * WARPS) {
-        const i64 tok = a.units == 1 ? unit : unit / a.units;
-        const int row0 = (int)(unit - tok * a.units) * a.per * HPW + sub;
-        const T* qrow = (const T*)a.q + tok * a.q_stride + e0;
-        const T* krow = (const T*)a.k + tok * a.k_stride + e0;
-        const T* vrow = (const T*)a.v + tok * a.v_stride + e0;
+    load_weights(sw, a.wq, a.wk, a.hd);
+    const int all = (int)a.tokens * a.units;
+    for (int unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += gridDim.x * WARPS) {
+        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per;
+        const int nq = a.gq - g0, nk = nq + a.gk;  // group g: a query group below nq, a key group below nk
+        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+        const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
+        const T* const v = (const T*)a.v + tok * a.v_stride + off - nk * step;
+        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0, hv = in ? a.hkv + nk * HPW - sub : 0;
         uint4 raw[UNIT];
 #pragma unroll
         for (int g = 0; g < UNIT; ++g) {
-            const int row = row0 + g * HPW, kr = row - a.h, vr = kr - a.hkv;
             raw[g] = make_uint4(0, 0, 0, 0);
-            if (g < a.per && in && row < rows)
-                raw[g] = *(const uint4*)(kr < 0 ? qrow + (i64)row * a.hd : vr < 0 ? krow + (i64)kr * a.hd : vrow + (i64)vr * a.hd);
+            if (g < a.per && g * HPW < (g < nq ? hq : g < nk ? hk : hv))
+                raw[g] = *(const uint4*)((g < nq ? q : g < nk ? k : v) + g * step);
         }
         i64 seq = 0;
         const int p = place::token_position(a.lens, a.cu, a.seqs, tok, seq);
         const i64 base = p >= 0 ? cache_row(a, seq, p) : -1;
-        float2 cs[V / 2];
-        if (in)
-#pragma unroll
-            for (int u = 0; u < V / 2; ++u) cs[u] = cos_sin<T>(p, f.turn[li * (V / 2) + u]);
-        T* qo = (T*)a.qo + tok * a.h * a.hd + e0;
+        Coef<T> c;
+        Turn<T> t;
+        if (g0 < a.gq + a.gk) t.at(p, f, e0 / 2);
+        if (nq > 0) c.of(t, sw[0] + e0);
+        T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
 #pragma unroll
         for (int g = 0; g < UNIT; ++g) {
             if (g >= a.per) break;
-            const int row = row0 + g * HPW, kr = row - a.h, vr = kr - a.hkv;
-            const bool on = in && row < rows;
-            float r = 1.f, x[V];
-            unpack<T, V>(raw[g], x);
-            if (norm) {
-                float ss = 0.f;
-#pragma unroll
-                for (int u = 0; u < V; ++u) ss = fmaf(x[u], x[u], ss);
-                r = rsqrtf(group_sum<LPH>(ss) / (float)a.hd + a.eps);
+            if (g == max(nq, 0) && g < nk) c.of(t, sw[1] + e0);
+            uint4 y = raw[g];
+            if (g < nk) y = norm_turn<T, LPH>(y, c, norm, a.inv_hd, a.eps);
+            if (g < nq) {
+                if (g * HPW < hq) *(uint4*)(qo + g * step) = p >= 0 ? y : make_uint4(0, 0, 0, 0);
+            } else if (base >= 0 && g * HPW < (g < nk ? hk : hv)) {
+                const int head = (g - (g < nk ? nq : nk)) * HPW + sub;
+                *(uint4*)((T*)(g < nk ? a.kc : a.vc) + base + (i64)head * a.page * a.hd + e0) = y;
             }
-            if (!on) continue;
-            if (vr < 0) {
-#pragma unroll
-                for (int u = 0; u < V; ++u) x[u] = p >= 0 ? x[u] * r * (kr < 0 ? wq[u] : wk[u]) : 0.f;
-                rotate<V>(x, cs);
-            }
-            if (kr < 0) stv<T, V>(qo + (i64)row * a.hd, x);
-            else if (base >= 0) stv<T, V>((T*)(vr < 0 ? a.kc : a.vc) + base + (i64)(vr < 0 ? kr : vr) * a.page * a.hd + e0, x);
         }
     }
 }
@@ -523,12 +622,16 @@ __global__ void __launch_bounds__(WARPS * 32) k_append_any(const __grid_constant
 }
 
 // ------------------------------------------------------------ launchers
-// Groups of HPW rows that a unit takes of one token: as many as fit (the
-// sines are then taken once a token), unless that would leave SMs without warps.
-static int groups_per_unit(Context* c, i64 tokens, int groups, int most) {
+// How a token's row groups are cut into units: as few as hold them (the sines
+// are then taken once a token), unless that would leave SMs without warps.
+// -> the grid of CTAs that walk the units, `per_sm` an SM at most.
+static int deal(Context* c, i64 tokens, int groups, int most, int per_sm, int& per, int& units) {
     const i64 want = (i64)c->sm_count * 16;
-    const int units = cdiv(groups, (int)std::max<i64>(1, std::min<i64>(most, tokens * groups / want)));
-    return cdiv(groups, units);
+    units = cdiv(groups, (int)std::max<i64>(1, std::min<i64>(most, tokens * groups / want)));
+    per = cdiv(groups, units);
+    units = cdiv(groups, per);
+    CATNN_CHECK(tokens * units <= 0x7fff0000, CATNN_ERR_SHAPE, "too many rows for one call");  // a grid's step more is an int too
+    return (int)std::min<i64>((tokens * units + WARPS - 1) / WARPS, c->sm_count * per_sm);
 }
 
 static int lanes_of(int hd, int vec) {
@@ -572,14 +675,13 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     check_heads(tokens, h, hkv, hd, "qk_norm_rope");
     if (tokens == 0) return;
     const Freq& f = freq_of(c, hd, theta);
-    FwdArgs a{q, k, q_stride, k_stride, wq, wk, pos, qo, ko, tokens, s, (int)h, (int)hkv, (int)hd, eps, 1, 1};
+    FwdArgs a{q, k, q_stride, k_stride, wq, wk, pos, qo, ko, tokens, s, (int)h, (int)hkv, (int)hd, eps, 1.f / (float)hd,
+              0, 1, 1};
     const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
     if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && aligned_to(qo, 16) &&
-        aligned_to(ko, 16) && aligned_to(wq, 16) && aligned_to(wk, 16)) {
-        const int groups = cdiv(h + hkv, 32 / lph);
-        a.per = groups_per_unit(c, tokens, groups, UNIT);
-        a.units = cdiv(groups, a.per);
-        const int grid = (int)std::min<i64>((tokens * a.units + WARPS - 1) / WARPS, c->sm_count * 3);
+        aligned_to(ko, 16)) {
+        a.gq = cdiv(h, 32 / lph);
+        const int grid = deal(c, tokens, a.gq + cdiv(hkv, 32 / lph), UNIT, 3, a.per, a.units);
 #define RUN(T, L) k_qk_fwd<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
@@ -592,12 +694,10 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
 }
 
 // CTAs of the adjoint: what the SMs hold at once, each walking many tokens,
-// because every CTA adds a row to the weight sums.
-static i64 qk_bwd_ctas(Context* c, i64 rows) { return std::min<i64>((i64)c->sm_count * 2, (rows + WARPS - 1) / WARPS); }
-
-// At least one CTA each for queries and keys, two rows a CTA where it has both.
+// because every CTA adds a row to each weight sum.
+constexpr int BWD_PER_SM = 2;
 size_t qk_norm_rope_bwd_workspace(Context* c, i64 b, i64 s, i64 h, i64 hkv, i64 hd) {
-    return (size_t)(qk_bwd_ctas(c, b * s * (h + hkv)) + 1) * 2 * hd * sizeof(float);
+    return (size_t)std::min<i64>((i64)c->sm_count * BWD_PER_SM, b * s * (h + hkv)) * 2 * hd * sizeof(float);
 }
 
 void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const float* wq, const float* wk,
@@ -608,31 +708,21 @@ void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     check_heads(tokens, h, hkv, hd, "qk_norm_rope backward");
     const Freq& f = freq_of(c, hd, theta);
     BwdArgs a{q, k, gq, gk, q_stride, k_stride, gq_stride, gk_stride, wq, wk, pos, dq, dk, work, tokens, s, (int)h, (int)hkv,
-              (int)hd, eps, {1, 1}, {1, 1}, 0};
-    int rows_q = 0, rows_k = 0;
+              (int)hd, eps, 1.f / (float)hd, 0, 1, 1};
+    int ctas = 0;
     if (tokens > 0) {
         const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
         if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && rows_ok(gq, gq_stride, hd, vec) &&
-            rows_ok(gk, gk_stride, hd, vec) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(wq, 16) &&
-            aligned_to(wk, 16)) {
-            const int groups[2] = {cdiv(h, 32 / lph), cdiv(hkv, 32 / lph)};
-            for (int m = 0; m < 2; ++m) {
-                a.per[m] = groups_per_unit(c, tokens, groups[m], BWD_UNIT);
-                a.units[m] = cdiv(groups[m], a.per[m]);
-            }
-            // CTAs in the proportion of the row groups, none without a unit
-            const i64 uq = tokens * a.units[0], uk = tokens * a.units[1], ctas = std::max<i64>(2, qk_bwd_ctas(c, uq + uk));
-            const i64 share = ctas * groups[0] / (groups[0] + groups[1]);
-            rows_q = (int)std::min<i64>(std::max<i64>(1, std::min(share, ctas - 1)), (uq + WARPS - 1) / WARPS);
-            rows_k = (int)std::min<i64>(ctas - rows_q, (uk + WARPS - 1) / WARPS);
-            a.q_ctas = rows_q;
-#define RUN(T, L) k_qk_bwd<T, L><<<rows_q + rows_k, WARPS * 32, 0, c->stream>>>(a, f)
+            rows_ok(gk, gk_stride, hd, vec) && aligned_to(dq, 16) && aligned_to(dk, 16)) {
+            a.groups_q = cdiv(h, 32 / lph);
+            ctas = deal(c, tokens, a.groups_q + cdiv(hkv, 32 / lph), BWD_UNIT, BWD_PER_SM, a.per, a.units);
+#define RUN(T, L) k_qk_bwd<T, L><<<ctas, WARPS * 32, 0, c->stream>>>(a, f)
             if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
         } else {
-            rows_q = rows_k = (int)qk_bwd_ctas(c, tokens * (h + hkv));
-            if (dtype == CATNN_BF16) k_qk_bwd_any<bf16><<<rows_q, WARPS * 32, 0, c->stream>>>(a, f);
-            else k_qk_bwd_any<float><<<rows_q, WARPS * 32, 0, c->stream>>>(a, f);
+            ctas = (int)std::min<i64>((i64)c->sm_count * BWD_PER_SM, (tokens * (h + hkv) + WARPS - 1) / WARPS);
+            if (dtype == CATNN_BF16) k_qk_bwd_any<bf16><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
+            else k_qk_bwd_any<float><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
         }
         launched(c);
     }
@@ -645,7 +735,7 @@ void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = tokens > 0 ? 1 : 0;  // with no tokens there is no first kernel that lets this one start
-    CUDA_OK(cudaLaunchKernelEx(&cfg, k_qk_dw, (const float*)work, rows_q, rows_k, (int)hd, dwq, dwk));
+    CUDA_OK(cudaLaunchKernelEx(&cfg, k_qk_dw, (const float*)work, ctas, (int)hd, dwq, dwk));
     launched(c);
 }
 
@@ -657,14 +747,13 @@ void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_str
     if (tokens == 0) return;
     const Freq& f = freq_of(c, hd, theta);
     AppendArgs a{q, k, v, q_stride, k_stride, v_stride, wq, wk, qo, kc, vc, table, lens, cu, tokens, seqs, (int)h, (int)hkv,
-                 (int)hd, (int)page, (int)max_pages, pages, eps, 1, 1, err};
+                 (int)hd, (int)page, (int)max_pages, pages, eps, 1.f / (float)hd, 0, 0, 1, 1, err};
     const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
     if (lph <= 32 && (!q || rows_ok(q, q_stride, hd, vec)) && rows_ok(k, k_stride, hd, vec) && rows_ok(v, v_stride, hd, vec) &&
-        aligned_to(qo, 16) && aligned_to(kc, 16) && aligned_to(vc, 16) && aligned_to(wq, 16) && aligned_to(wk, 16)) {
-        const int groups = cdiv(h + 2 * hkv, 32 / lph);
-        a.per = groups_per_unit(c, tokens, groups, UNIT);
-        a.units = cdiv(groups, a.per);
-        const int grid = (int)std::min<i64>((tokens * a.units + WARPS - 1) / WARPS, c->sm_count * 3);
+        aligned_to(qo, 16) && aligned_to(kc, 16) && aligned_to(vc, 16)) {
+        a.gq = cdiv(h, 32 / lph);
+        a.gk = cdiv(hkv, 32 / lph);
+        const int grid = deal(c, tokens, a.gq + 2 * a.gk, UNIT, 3, a.per, a.units);
 #define RUN(T, L) k_append<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN

@@ -15,29 +15,45 @@ namespace place {
 
 typedef int64_t i64;
 
-// Position of new token t, its last `cu[seq+1] - cu[seq]` ones being a
-// sequence's new tokens (cu null: token t is sequence t's only one), and the
-// sequence it belongs to. -1 when it belongs to none: a row before the first
-// or behind the last sequence, or one whose sequence ends before position 0.
-PLACE_FN int token_position(const int32_t* lens, const int32_t* cu, i64 seqs, i64 t, i64& seq) {
-    i64 end = t + 1;
-    seq = t;
-    if (cu) {
-        if (seqs < 1 || t < cu[0] || t >= cu[seqs]) return -1;
-        i64 lo = 0, hi = seqs;  // the last sequence whose first token is at or before t
-        while (hi - lo > 1) {
-            const i64 mid = (lo + hi) >> 1;
-            if (cu[mid] <= t) lo = mid;
-            else hi = mid;
+// The sequence of a new token, for tokens met in ascending order. A
+// sequence's new tokens are rows [cu[seq], cu[seq + 1]), its last positions (cu
+// null: token t is sequence t's only one).
+struct Token {
+    int seq = -1, end = -1;  // the sequence, and the row behind its last new token; seq < 0: none
+    int len = 0;
+    PLACE_FN void move_to(const int32_t* lens, const int32_t* cu, int seqs, int t) {
+        if (seq >= 0 && t < end) return;
+        seq = -1;
+        if (!cu) {
+            if (t >= seqs) return;
+            seq = t;
+            end = t + 1;
+        } else {
+            if (seqs < 1 || t < cu[0] || t >= cu[seqs]) return;
+            int lo = 0, hi = seqs;  // the last sequence whose first token is at or before t
+            while (hi - lo > 1) {
+                const int mid = lo + ((hi - lo) >> 1);
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            end = cu[lo + 1];
+            if (end <= t) return;  // starts that do not ascend
+            seq = lo;
         }
-        seq = lo;
-        end = cu[lo + 1];
-        if (end <= t) return -1;  // starts that do not ascend
-    } else if (t >= seqs) {
-        return -1;
+        len = lens[seq];
     }
-    const i64 pos = (i64)lens[seq] - (end - t);
-    return pos < 0 ? -1 : (int)pos;
+    // Its position, or -1 when it has none: a row before the first or behind
+    // the last sequence, or one whose sequence ends before position 0.
+    PLACE_FN int position(int t) const {
+        const i64 pos = (i64)len - ((i64)end - t);
+        return seq < 0 || pos < 0 ? -1 : (int)pos;
+    }
+};
+PLACE_FN int token_position(const int32_t* lens, const int32_t* cu, int seqs, int t, int& seq) {
+    Token at;
+    at.move_to(lens, cu, seqs, t);
+    seq = at.seq;
+    return at.position(t);
 }
 
 // Index of the first element of kv head 0 at a position: caches [pages, hkv,

@@ -194,6 +194,35 @@ __device__ __forceinline__ void load_weights(float (&sw)[2][MAX_HD], const float
     __syncthreads();
 }
 
+// How the row groups of all tokens are dealt out to the warps of a grid: a
+// token's groups to `parts` warps, `per` to each. Such a team takes every
+// teams-th token (run = 0: all warps then read along one front, 17.1 us where
+// runs took 18.1 for 16384 tokens of 16 + 4 heads of 64), or a run of
+// neighbours, where one look-up serves many (the append: 39 against 43 us).
+struct Deal {
+    int tokens, groups, parts, per, run, teams;
+};
+struct Share {
+    int t0, t1, dt, g0, g1;
+};
+__device__ __forceinline__ Share share_of(const Deal& d) {
+    const int w = blockIdx.x * WARPS + (threadIdx.x >> 5), team = w / d.parts, part = w - team * d.parts;
+    Share s;
+    if (team >= d.teams) {
+        s.t0 = s.t1 = 0;
+    } else if (d.run == 0) {
+        s.t0 = team;
+        s.t1 = d.tokens;
+    } else {
+        s.t0 = (int)min((i64)d.tokens, (i64)team * d.run);
+        s.t1 = (int)min((i64)d.tokens, (i64)s.t0 + d.run);
+    }
+    s.dt = d.run == 0 ? d.teams : 1;
+    s.g0 = part * d.per;
+    s.g1 = min(d.groups, s.g0 + d.per);
+    return s;
+}
+
 struct FwdArgs {
     const void *q, *k;
     i64 q_stride, k_stride;  // elements between tokens
@@ -203,15 +232,14 @@ struct FwdArgs {
     i64 tokens, s;
     int h, hkv, hd;
     float eps, inv_hd;
-    // row groups of a token: gq of its query heads, then those of its key
-    // heads; a unit is `per` of them, `units` units a token
-    int gq, per, units;
+    Deal deal;
+    int gq;  // row groups of a token: gq of its query heads, then those of its key heads
 };
 
 // Forward on 16-byte pieces. A group is the HPW = 32 / LPH heads that a warp
-// takes at once. A warp walks the units in grid order; all rows of a unit are
-// on their way before its sines are taken.
-constexpr int UNIT = 6;  // row groups of a unit, at most
+// takes at once. A warp walks its tokens, and each one's groups a batch at a
+// time; a batch's rows are all on their way before the token's sines are taken.
+constexpr int BATCH = 6;
 template <typename T, int LPH>
 __global__ void __launch_bounds__(WARPS * 32, 3) k_qk_fwd(const __grid_constant__ FwdArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, HPW = 32 / LPH;
@@ -219,31 +247,32 @@ __global__ void __launch_bounds__(WARPS * 32, 3) k_qk_fwd(const __grid_constant_
     const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd;
     load_weights(sw, a.wq, a.wk, a.hd);
-    const int all = (int)a.tokens * a.units;
-    for (int unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += gridDim.x * WARPS) {
-        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per, nq = a.gq - g0;
-        // group g is a query group for g < nq
-        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
-        const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
-        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;  // group g is there for g·HPW below
-        uint4 raw[UNIT];
-#pragma unroll
-        for (int g = 0; g < UNIT; ++g) {
-            raw[g] = make_uint4(0, 0, 0, 0);
-            if (g < a.per && g * HPW < (g < nq ? hq : hk)) raw[g] = *(const uint4*)((g < nq ? q : k) + g * step);
-        }
+    const Share w = share_of(a.deal);
+    for (int tok = w.t0; tok < w.t1; tok += w.dt) {
         Turn<T> t;
-        t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
-        T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
-        T* const ko = (T*)a.ko + (i64)tok * a.hkv * a.hd + off - nq * step;
-        Coef<T> c;
-        if (nq > 0) c.of(t, sw[0] + e0);
+        for (int g0 = w.g0; g0 < w.g1; g0 += BATCH) {
+            const int nq = a.gq - g0, n = w.g1 - g0;  // group g is a query group for g < nq
+            const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+            const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
+            const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;  // group g is there for g·HPW below
+            uint4 raw[BATCH];
 #pragma unroll
-        for (int g = 0; g < UNIT; ++g) {
-            if (g >= a.per) break;
-            if (g == max(nq, 0)) c.of(t, sw[1] + e0);
-            const uint4 y = norm_turn<T, LPH>(raw[g], c, true, a.inv_hd, a.eps);
-            if (g * HPW < (g < nq ? hq : hk)) *(uint4*)((g < nq ? qo : ko) + g * step) = y;
+            for (int g = 0; g < BATCH; ++g) {
+                raw[g] = make_uint4(0, 0, 0, 0);
+                if (g < n && g * HPW < (g < nq ? hq : hk)) raw[g] = *(const uint4*)((g < nq ? q : k) + g * step);
+            }
+            if (g0 == w.g0) t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
+            T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
+            T* const ko = (T*)a.ko + (i64)tok * a.hkv * a.hd + off - nq * step;
+            Coef<T> c;
+            if (nq > 0) c.of(t, sw[0] + e0);
+#pragma unroll
+            for (int g = 0; g < BATCH; ++g) {
+                if (g >= n) break;
+                if (g == max(nq, 0)) c.of(t, sw[1] + e0);
+                const uint4 y = norm_turn<T, LPH>(raw[g], c, true, a.inv_hd, a.eps);
+                if (g * HPW < (g < nq ? hq : hk)) *(uint4*)((g < nq ? qo : ko) + g * step) = y;
+            }
         }
     }
 }
@@ -297,12 +326,13 @@ struct BwdArgs {
     i64 tokens, s;
     int h, hkv, hd;
     float eps, inv_hd;
-    int groups_q, per, units;  // as in the forward
+    Deal deal;
+    int groups_q;  // as in the forward
 };
 
-// Adjoint on 16-byte pieces, units as in the forward; both weight sums stay in
-// registers over all units of a warp.
-constexpr int BWD_UNIT = 5;
+// Adjoint on 16-byte pieces, dealt out as the forward; both weight sums stay
+// in registers over all of a warp's rows.
+constexpr int BWD_BATCH = 5;
 template <typename T, int LPH>
 __global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant__ BwdArgs a, const __grid_constant__ Freq f) {
     constexpr int V = VEC<T>, N = NP<T>, HPW = 32 / LPH;
@@ -318,35 +348,39 @@ __global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant_
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[m][0][j] = acc[m][1][j] = pack2(0.f, 0.f);
-    const int all = (int)a.tokens * a.units;
-    for (int unit = blockIdx.x * WARPS + warp; unit < all; unit += gridDim.x * WARPS) {
-        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per, nq = a.groups_q - g0;
-        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+    const f2 minus = pack2(-1.f, -1.f);
+    const Share w = share_of(a.deal);
+    for (int tok = w.t0; tok < w.t1; tok += w.dt) {
+      Turn<T> t;
+      f2 ns[N];
+      for (int b0 = w.g0; b0 < w.g1; b0 += BWD_BATCH) {
+        const int nq = a.groups_q - b0, n = w.g1 - b0;
+        const T* const q = (const T*)a.q + tok * a.q_stride + off + b0 * step;
         const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
-        const T* const gq = (const T*)a.gq + tok * a.gq_stride + off + g0 * step;
+        const T* const gq = (const T*)a.gq + tok * a.gq_stride + off + b0 * step;
         const T* const gk = (const T*)a.gk + tok * a.gk_stride + off - nq * step;
-        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;
-        uint4 xr[BWD_UNIT], yr[BWD_UNIT];
+        const int hq = in ? a.h - b0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;
+        uint4 xr[BWD_BATCH], yr[BWD_BATCH];
 #pragma unroll
-        for (int g = 0; g < BWD_UNIT; ++g) {
+        for (int g = 0; g < BWD_BATCH; ++g) {
             xr[g] = yr[g] = make_uint4(0, 0, 0, 0);
-            if (g < a.per && g * HPW < (g < nq ? hq : hk)) {
+            if (g < n && g * HPW < (g < nq ? hq : hk)) {
                 xr[g] = *(const uint4*)((g < nq ? q : k) + g * step);
                 yr[g] = *(const uint4*)((g < nq ? gq : gk) + g * step);
             }
         }
-        Turn<T> t;
-        t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
-        T* const dq = (T*)a.dq + (i64)tok * a.h * a.hd + off + g0 * step;
-        T* const dk = (T*)a.dk + (i64)tok * a.hkv * a.hd + off - nq * step;
-        const f2 minus = pack2(-1.f, -1.f);
-        f2 ns[N], w0[N], w1[N];
+        if (b0 == w.g0) {
+            t.at(a.pos ? a.pos[tok] : (int)((unsigned)tok % (unsigned)a.s), f, e0 / 2);
 #pragma unroll
-        for (int j = 0; j < N; ++j) ns[j] = mul2(t.s[j], minus);
+            for (int j = 0; j < N; ++j) ns[j] = mul2(t.s[j], minus);
+        }
+        T* const dq = (T*)a.dq + (i64)tok * a.h * a.hd + off + b0 * step;
+        T* const dk = (T*)a.dk + (i64)tok * a.hkv * a.hd + off - nq * step;
+        f2 w0[N], w1[N];
         weights<T>(sw[nq > 0 ? 0 : 1] + e0, w0, w1);
 #pragma unroll
-        for (int g = 0; g < BWD_UNIT; ++g) {
-            if (g >= a.per) break;
+        for (int g = 0; g < BWD_BATCH; ++g) {
+            if (g >= n) break;
             if (g > 0 && g == nq) weights<T>(sw[1] + e0, w0, w1);
             f2 x0[N], x1[N], y0[N], y1[N], g0_[N], g1_[N];
             unpack<T>(xr[g], x0, x1);
@@ -384,6 +418,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant_
             }
             if (on) *(uint4*)((g < nq ? dq : dk) + g * step) = repack<T>(y0, y1);
         }
+      }
     }
     // the groups of a warp, then the warps of the CTA, each in a fixed order
 #pragma unroll
@@ -511,12 +546,13 @@ struct AppendArgs {
     int h, hkv, hd, page, max_pages;
     i64 pages;
     float eps, inv_hd;
-    int gq, gk, per, units;
+    Deal deal;
+    int gq, gk;
     int* err;
 };
 
 // The cache row of (seq, pos), kv head 0, or -1 (and *err set) where there is none.
-__device__ __forceinline__ i64 cache_row(const AppendArgs& a, i64 seq, int pos) {
+__device__ __forceinline__ i64 cache_row(const AppendArgs& a, int seq, int pos) {
     const i64 at = place::cache_index(a.table, seq, pos, a.page, a.max_pages, a.pages, a.hkv, a.hd);
     if (at < 0 && a.err) atomicExch(a.err, 1);
     return at;
@@ -534,40 +570,47 @@ __global__ void __launch_bounds__(WARPS * 32, 3) k_append(const __grid_constant_
     const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd, norm = a.wq != nullptr;
     load_weights(sw, a.wq, a.wk, a.hd);
-    const int all = (int)a.tokens * a.units;
-    for (int unit = blockIdx.x * WARPS + (threadIdx.x >> 5); unit < all; unit += gridDim.x * WARPS) {
-        const int tok = a.units == 1 ? unit : unit / a.units, g0 = (unit - tok * a.units) * a.per;
-        const int nq = a.gq - g0, nk = nq + a.gk;  // group g: a query group below nq, a key group below nk
-        const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
-        const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
-        const T* const v = (const T*)a.v + tok * a.v_stride + off - nk * step;
-        const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0, hv = in ? a.hkv + nk * HPW - sub : 0;
-        uint4 raw[UNIT];
-#pragma unroll
-        for (int g = 0; g < UNIT; ++g) {
-            raw[g] = make_uint4(0, 0, 0, 0);
-            if (g < a.per && g * HPW < (g < nq ? hq : g < nk ? hk : hv))
-                raw[g] = *(const uint4*)((g < nq ? q : g < nk ? k : v) + g * step);
-        }
-        i64 seq = 0;
-        const int p = place::token_position(a.lens, a.cu, a.seqs, tok, seq);
-        const i64 base = p >= 0 ? cache_row(a, seq, p) : -1;
-        Coef<T> c;
+    const Share w = share_of(a.deal);
+    place::Token at;
+    for (int tok = w.t0; tok < w.t1; tok += w.dt) {
         Turn<T> t;
-        if (g0 < a.gq + a.gk) t.at(p, f, e0 / 2);
-        if (nq > 0) c.of(t, sw[0] + e0);
-        T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
+        int p = -1;
+        i64 base = -1;
+        for (int g0 = w.g0; g0 < w.g1; g0 += BATCH) {
+            const int nq = a.gq - g0, nk = nq + a.gk, n = w.g1 - g0;  // group g: a query group below nq, a key group below nk
+            const T* const q = (const T*)a.q + tok * a.q_stride + off + g0 * step;
+            const T* const k = (const T*)a.k + tok * a.k_stride + off - nq * step;
+            const T* const v = (const T*)a.v + tok * a.v_stride + off - nk * step;
+            const int hq = in ? a.h - g0 * HPW - sub : 0, hk = in ? a.hkv + nq * HPW - sub : 0;
+            const int hv = in ? a.hkv + nk * HPW - sub : 0;
+            uint4 raw[BATCH];
 #pragma unroll
-        for (int g = 0; g < UNIT; ++g) {
-            if (g >= a.per) break;
-            if (g == max(nq, 0) && g < nk) c.of(t, sw[1] + e0);
-            uint4 y = raw[g];
-            if (g < nk) y = norm_turn<T, LPH>(y, c, norm, a.inv_hd, a.eps);
-            if (g < nq) {
-                if (g * HPW < hq) *(uint4*)(qo + g * step) = p >= 0 ? y : make_uint4(0, 0, 0, 0);
-            } else if (base >= 0 && g * HPW < (g < nk ? hk : hv)) {
-                const int head = (g - (g < nk ? nq : nk)) * HPW + sub;
-                *(uint4*)((T*)(g < nk ? a.kc : a.vc) + base + (i64)head * a.page * a.hd + e0) = y;
+            for (int g = 0; g < BATCH; ++g) {
+                raw[g] = make_uint4(0, 0, 0, 0);
+                if (g < n && g * HPW < (g < nq ? hq : g < nk ? hk : hv))
+                    raw[g] = *(const uint4*)((g < nq ? q : g < nk ? k : v) + g * step);
+            }
+            if (g0 == w.g0) {
+                at.move_to(a.lens, a.cu, (int)a.seqs, tok);
+                p = at.position(tok);
+                base = p >= 0 ? cache_row(a, at.seq, p) : -1;
+                if (g0 < a.gq + a.gk) t.at(p, f, e0 / 2);
+            }
+            Coef<T> c;
+            if (nq > 0) c.of(t, sw[0] + e0);
+            T* const qo = (T*)a.qo + (i64)tok * a.h * a.hd + off + g0 * step;
+#pragma unroll
+            for (int g = 0; g < BATCH; ++g) {
+                if (g >= n) break;
+                if (g == max(nq, 0) && g < nk) c.of(t, sw[1] + e0);
+                uint4 y = raw[g];
+                if (g < nk) y = norm_turn<T, LPH>(y, c, norm, a.inv_hd, a.eps);
+                if (g < nq) {
+                    if (g * HPW < hq) *(uint4*)(qo + g * step) = p >= 0 ? y : make_uint4(0, 0, 0, 0);
+                } else if (base >= 0 && g * HPW < (g < nk ? hk : hv)) {
+                    const int head = (g - (g < nk ? nq : nk)) * HPW + sub;
+                    *(uint4*)((T*)(g < nk ? a.kc : a.vc) + base + (i64)head * a.page * a.hd + e0) = y;
+                }
             }
         }
     }
@@ -581,8 +624,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_append_any(const __grid_constant
     if (tok >= a.tokens) return;
     const int row = (int)(unit - tok * rows);
     const int kind = row < a.h ? 0 : row < a.h + a.hkv ? 1 : 2, head = kind == 0 ? row : kind == 1 ? row - a.h : row - a.h - a.hkv;
-    i64 seq = 0;
-    const int p = place::token_position(a.lens, a.cu, a.seqs, tok, seq);
+    int seq = 0;
+    const int p = place::token_position(a.lens, a.cu, (int)a.seqs, (int)tok, seq);
     const i64 base = p >= 0 ? cache_row(a, seq, p) : -1;
     if (kind != 0 && base < 0) return;
     const T* x = kind == 0 ? (const T*)a.q + tok * a.q_stride : kind == 1 ? (const T*)a.k + tok * a.k_stride : (const T*)a.v + tok * a.v_stride;
@@ -622,16 +665,19 @@ __global__ void __launch_bounds__(WARPS * 32) k_append_any(const __grid_constant
 }
 
 // ------------------------------------------------------------ launchers
-// How a token's row groups are cut into units: as few as hold them (the sines
-// are then taken once a token), unless that would leave SMs without warps.
-// -> the grid of CTAs that walk the units, `per_sm` an SM at most.
-static int deal(Context* c, i64 tokens, int groups, int most, int per_sm, int& per, int& units) {
-    const i64 want = (i64)c->sm_count * 16;
-    units = cdiv(groups, (int)std::max<i64>(1, std::min<i64>(most, tokens * groups / want)));
-    per = cdiv(groups, units);
-    units = cdiv(groups, per);
-    CATNN_CHECK(tokens * units <= 0x7fff0000, CATNN_ERR_SHAPE, "too many rows for one call");  // a grid's step more is an int too
-    return (int)std::min<i64>((tokens * units + WARPS - 1) / WARPS, c->sm_count * per_sm);
+// A warp takes all groups of its tokens (whose sines and places are then found
+// once a token) unless that would leave SMs without warps. -> the grid, up to
+// `per_sm` CTAs an SM.
+static int deal_out(Context* c, i64 tokens, int groups, int per_sm, bool runs, Deal& d) {
+    const i64 want = (i64)c->sm_count * 16, most = (i64)c->sm_count * per_sm;
+    d.tokens = (int)tokens;
+    d.groups = groups;
+    d.per = (int)std::max<i64>(1, std::min<i64>(groups, tokens * groups / want));
+    d.parts = cdiv(groups, d.per);
+    const i64 ctas = std::min(most, (tokens * d.parts + WARPS - 1) / WARPS);
+    d.teams = (int)std::max<i64>(1, std::min(tokens, ctas * WARPS / d.parts));
+    d.run = runs ? cdiv(tokens, d.teams) : 0;
+    return (int)(((i64)d.teams * d.parts + WARPS - 1) / WARPS);
 }
 
 static int lanes_of(int hd, int vec) {
@@ -643,7 +689,7 @@ static int lanes_of(int hd, int vec) {
 static void check_heads(i64 tokens, i64 h, i64 hkv, i64 hd, const char* what) {
     CATNN_CHECK(hd >= 2 && hd % 2 == 0 && hd <= MAX_HD, CATNN_ERR_UNSUPPORTED,
                 std::string(what) + ": head_dim must be even and at most 256");
-    CATNN_CHECK(tokens >= 0 && h >= 0 && hkv >= 1 && h + 2 * hkv <= 65536 && tokens <= (1ll << 31) - 1, CATNN_ERR_SHAPE,
+    CATNN_CHECK(tokens >= 0 && h >= 0 && hkv >= 1 && h + 2 * hkv <= 65536 && tokens <= 0x7fff0000, CATNN_ERR_SHAPE,
                 std::string(what) + ": sizes");
 }
 static int grid_of(i64 warps, const char* what) {
@@ -676,12 +722,12 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     if (tokens == 0) return;
     const Freq& f = freq_of(c, hd, theta);
     FwdArgs a{q, k, q_stride, k_stride, wq, wk, pos, qo, ko, tokens, s, (int)h, (int)hkv, (int)hd, eps, 1.f / (float)hd,
-              0, 1, 1};
+              {}, 0};
     const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
     if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && aligned_to(qo, 16) &&
         aligned_to(ko, 16)) {
         a.gq = cdiv(h, 32 / lph);
-        const int grid = deal(c, tokens, a.gq + cdiv(hkv, 32 / lph), UNIT, 3, a.per, a.units);
+        const int grid = deal_out(c, tokens, a.gq + cdiv(hkv, 32 / lph), 3, false, a.deal);
 #define RUN(T, L) k_qk_fwd<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
@@ -708,14 +754,14 @@ void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     check_heads(tokens, h, hkv, hd, "qk_norm_rope backward");
     const Freq& f = freq_of(c, hd, theta);
     BwdArgs a{q, k, gq, gk, q_stride, k_stride, gq_stride, gk_stride, wq, wk, pos, dq, dk, work, tokens, s, (int)h, (int)hkv,
-              (int)hd, eps, 1.f / (float)hd, 0, 1, 1};
+              (int)hd, eps, 1.f / (float)hd, {}, 0};
     int ctas = 0;
     if (tokens > 0) {
         const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
         if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && rows_ok(gq, gq_stride, hd, vec) &&
             rows_ok(gk, gk_stride, hd, vec) && aligned_to(dq, 16) && aligned_to(dk, 16)) {
             a.groups_q = cdiv(h, 32 / lph);
-            ctas = deal(c, tokens, a.groups_q + cdiv(hkv, 32 / lph), BWD_UNIT, BWD_PER_SM, a.per, a.units);
+            ctas = deal_out(c, tokens, a.groups_q + cdiv(hkv, 32 / lph), BWD_PER_SM, false, a.deal);
 #define RUN(T, L) k_qk_bwd<T, L><<<ctas, WARPS * 32, 0, c->stream>>>(a, f)
             if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
@@ -747,13 +793,13 @@ void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_str
     if (tokens == 0) return;
     const Freq& f = freq_of(c, hd, theta);
     AppendArgs a{q, k, v, q_stride, k_stride, v_stride, wq, wk, qo, kc, vc, table, lens, cu, tokens, seqs, (int)h, (int)hkv,
-                 (int)hd, (int)page, (int)max_pages, pages, eps, 1.f / (float)hd, 0, 0, 1, 1, err};
+                 (int)hd, (int)page, (int)max_pages, pages, eps, 1.f / (float)hd, {}, 0, 0, err};
     const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
     if (lph <= 32 && (!q || rows_ok(q, q_stride, hd, vec)) && rows_ok(k, k_stride, hd, vec) && rows_ok(v, v_stride, hd, vec) &&
         aligned_to(qo, 16) && aligned_to(kc, 16) && aligned_to(vc, 16)) {
         a.gq = cdiv(h, 32 / lph);
         a.gk = cdiv(hkv, 32 / lph);
-        const int grid = deal(c, tokens, a.gq + 2 * a.gk, UNIT, 3, a.per, a.units);
+        const int grid = deal_out(c, tokens, a.gq + 2 * a.gk, 3, true, a.deal);
 #define RUN(T, L) k_append<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN

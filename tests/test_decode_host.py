@@ -13,8 +13,15 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 SHIM = '''
 #include "paged_place.cuh"
-extern "C" int position(const int32_t* lens, const int32_t* cu, int64_t seqs, int64_t t, int64_t* seq) {
+extern "C" int position(const int32_t* lens, const int32_t* cu, int seqs, int t, int* seq) {
     return catnn::place::token_position(lens, cu, seqs, t, *seq);
+}
+extern "C" void positions(const int32_t* lens, const int32_t* cu, int seqs, int t0, int t1, int* out) {
+    catnn::place::Token at;  // as a kernel's warp walks its rows
+    for (int t = t0; t < t1; ++t) {
+        at.move_to(lens, cu, seqs, t);
+        out[t - t0] = at.position(t);
+    }
 }
 extern "C" int64_t cache_at(const int32_t* table, int64_t seq, int pos, int page, int max_pages, int64_t pages, int hkv,
                             int hd) {
@@ -32,7 +39,9 @@ def place(tmp_path_factory):
                     str(so)], check=True)
     lib = C.CDLL(str(so))
     I32P = C.POINTER(C.c_int32)
-    lib.position.argtypes = [I32P, I32P, C.c_int64, C.c_int64, C.POINTER(C.c_int64)]
+    lib.position.argtypes = [I32P, I32P, C.c_int, C.c_int, I32P]
+    lib.positions.argtypes = [I32P, I32P, C.c_int, C.c_int, C.c_int, I32P]
+    lib.positions.restype = None
     lib.cache_at.argtypes = [I32P, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int]
     lib.cache_at.restype = C.c_int64
     return lib
@@ -46,7 +55,7 @@ def test_positions_of_ragged_new_tokens(place):
     cu, lens = [2, 5, 5, 6, 10], [7, 4, 1, 3]  # sequence 1 has no new token, 3 more than its length
     got = []
     for t in range(12):
-        seq = C.c_int64(-7)
+        seq = C.c_int32(-7)
         p = place.position(ints(*lens), ints(*cu), 4, t, C.byref(seq))
         got.append((p, seq.value) if p >= 0 else p)
     # rows 0, 1 lie before the first sequence, 10, 11 behind the last; row 6 would be position -1
@@ -54,7 +63,7 @@ def test_positions_of_ragged_new_tokens(place):
 
 
 def test_positions_of_single_tokens_and_bad_starts(place):
-    seq = C.c_int64()
+    seq = C.c_int32()
     assert [place.position(ints(5, 0, -3, 1), None, 4, t, C.byref(seq)) for t in range(5)] == [4, -1, -1, 0, -1]
     assert place.position(ints(), ints(0), 0, 0, C.byref(seq)) == -1  # no sequences at all
     # starts that do not ascend name no sequence, and never an index out of [0, seqs)
@@ -63,12 +72,31 @@ def test_positions_of_single_tokens_and_bad_starts(place):
         n = int(r.integers(1, 6))
         cu, lens = r.integers(-5, 15, n + 1), r.integers(-5, 40, n)
         t = int(r.integers(0, 20))
-        seq = C.c_int64(0)
+        seq = C.c_int32(0)
         p = place.position(ints(*map(int, lens)), ints(*map(int, cu)), n, t, C.byref(seq))
         assert p >= -1
         if p >= 0:
             assert 0 <= seq.value < n and cu[seq.value] <= t < cu[seq.value + 1]
             assert p == lens[seq.value] - (cu[seq.value + 1] - t)
+
+
+def test_positions_of_a_walk(place):
+    """A walk over rows, from anywhere, finds what a look-up of each finds."""
+    r = np.random.default_rng(1)
+    for _ in range(300):
+        n = int(r.integers(1, 9))
+        cu = np.concatenate([[0], np.cumsum(r.integers(0, 6, n))]) + int(r.integers(0, 3))
+        lens = ints(*map(int, r.integers(-2, 12, n)))
+        c = ints(*map(int, cu))
+        t0, t1 = sorted(map(int, r.integers(0, 30, 2)))
+        out = ints(*([0] * (t1 - t0)))
+        place.positions(lens, c, n, t0, t1, out)
+        seq = C.c_int32()
+        assert list(out)[:t1 - t0] == [place.position(lens, c, n, t, C.byref(seq)) for t in range(t0, t1)]
+    # lengths at the ends of their type do not wrap around
+    big = 2 ** 31 - 1
+    assert place.position(ints(-big - 1), ints(0, big), 1, 0, C.byref(seq)) == -1
+    assert place.position(ints(big), ints(0, big), 1, big - 1, C.byref(seq)) == big - 1
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 128])

@@ -129,12 +129,20 @@ __global__ void __launch_bounds__(THREADS) k_down_any(const __grid_constant__ Ar
 // expert, whose first tiles are fetched while the first kernel routes, and
 // the second kernel, whose first tiles are fetched beside the first's last,
 // reads what the first found (ALL = true).
-constexpr int BK = 64, XPITCH = 144;
-constexpr int SMEM_MAX = 128 * 1024;  // the widest ring and what lies beside it
+//
+// fp32 (multiples of 4) runs the same kernels with other hands: the tensor
+// cores would round to TF32, so lanes are columns and packed FMAs multiply,
+// two k at a time; a warp has one of the matrices and its share of a tile's
+// rows. Its logits are TF32 products all the same, of both halves of every
+// value (a 21-bit product, as exact as the fp32 sums that it goes into).
+constexpr int BK = 64;
+template <typename T> constexpr int XPITCH = BK * (int)sizeof(T) + 16;
+template <typename T> constexpr int PIECE = 16 / (int)sizeof(T);
+constexpr int SMEM_MAX = 144 * 1024;  // the widest ring and what lies beside it
 
 struct TcArgs {
-    const bf16 *x, *gate;
-    bf16 *h, *y;
+    const void *x, *gate;
+    void *h, *y;
     float* yp;        // [runs][T·k, hidden]: each pair's share of y from each run of rows, before its weight
     unsigned* taken;  // [T], then [T·k] weights: what the first kernel found (ALL)
     unsigned* count;  // [column tiles of hidden]: CTAs that have put theirs there
@@ -196,7 +204,60 @@ __device__ __forceinline__ unsigned choose(float l, int E, int k, int lane, floa
 
 // `issued` is called by every warp when its first batch's loads are on their way.
 template <int R8, int CW, typename Issued>
-__device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, char* gs, float* part, Issued issued) {
+__device__ __forceinline__ void logits_f32(const TcArgs& a, int t0, int rows, float* part, Issued issued) {
+    constexpr int NB = 4;  // runs of 16 k in flight
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, kj = (lane & 3) * 4;
+    const int nt = (a.E + 7) / 8, ep = nt * 8;
+    const float* xrow[R8];
+#pragma unroll
+    for (int i = 0; i < R8; ++i) xrow[i] = (const float*)a.x + (i64)(t0 + min(i * 8 + row, rows - 1)) * a.hidden + kj;
+#pragma unroll 1
+    for (int j = 0; j < nt; ++j) {
+        const float* gcol = (const float*)a.gate + (i64)kj * a.E + min(j * 8 + row, a.E - 1);
+        float acc[4] = {}, low[4] = {};
+#pragma unroll 1
+        for (int k0 = warp * 16; k0 < a.hidden; k0 += NB * CW * 16) {
+            float x[NB][R8][4], g[NB][4];
+#pragma unroll
+            for (int q = 0; q < NB; ++q) {
+                const int k1 = k0 + q * CW * 16;
+                const bool on = k1 + kj < a.hidden;  // hidden is a multiple of 4
+#pragma unroll
+                for (int i = 0; i < R8; ++i) {
+                    const float4 v = on ? *(const float4*)(xrow[i] + k1) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[q][i][0] = v.x, x[q][i][1] = v.y, x[q][i][2] = v.z, x[q][i][3] = v.w;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) g[q][u] = on ? gcol[(i64)(k1 + u) * a.E] : 0.f;
+            }
+            if (j == 0 && k0 == warp * 16) issued();
+#pragma unroll
+            for (int q = 0; q < NB; ++q)
+#pragma unroll
+                for (int v = 0; v < 4; v += 2) {  // the instruction's k and k + 4 are a lane's two neighbours
+                    uint32_t ah[4] = {}, al[4] = {}, bh[2], bl[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                        for (int i = 0; i < R8; ++i) {
+                            ah[u * 2 + i] = tc::to_tf32(x[q][i][v + u]);
+                            al[u * 2 + i] = tc::to_tf32(x[q][i][v + u] - __uint_as_float(ah[u * 2 + i]));
+                        }
+                        bh[u] = tc::to_tf32(g[q][v + u]);
+                        bl[u] = tc::to_tf32(g[q][v + u] - __uint_as_float(bh[u]));
+                    }
+                    tc::mma1688_tf32(acc, ah, bh[0], bh[1]);
+                    tc::mma1688_tf32(low, ah, bl[0], bl[1]);
+                    tc::mma1688_tf32(low, al, bh[0], bh[1]);
+                }
+        }
+        float* p = part + (warp * RT + row) * ep + j * 8 + (lane & 3) * 2;
+        *(float2*)p = make_float2(acc[0] + low[0], acc[1] + low[1]);
+        if (R8 > 1) *(float2*)(p + 8 * ep) = make_float2(acc[2] + low[2], acc[3] + low[3]);
+    }
+}
+template <int R8, int CW, typename Issued>
+__device__ __forceinline__ void logits_bf16(const TcArgs& a, int t0, int rows, char* gs, float* part, Issued issued) {
     constexpr int NB = R8 == 1 ? 8 : 4;  // runs of 32 k in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, kj = (lane & 3) * 8;
     const int nt = (a.E + 7) / 8, ep = nt * 8;
@@ -204,7 +265,7 @@ __device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, cha
     const uint32_t gaddr = tc::smem_u32(gs) + (8 * ((lane & 7) >> 1) + (lane & 1) + 2 * (lane >> 3)) * 16;
     const bf16* xrow[R8];
 #pragma unroll
-    for (int i = 0; i < R8; ++i) xrow[i] = a.x + (i64)(t0 + min(i * 8 + row, rows - 1)) * a.hidden + kj;  // a row past the last is not used
+    for (int i = 0; i < R8; ++i) xrow[i] = (const bf16*)a.x + (i64)(t0 + min(i * 8 + row, rows - 1)) * a.hidden + kj;  // a row past the last is not used
     // (the code is kept short: a launch meets its instructions cold, and their fetching costs as much as the data's)
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
@@ -220,7 +281,7 @@ __device__ __forceinline__ void logits_tc(const TcArgs& a, int t0, int rows, cha
                     x[q][i] = k1 + kj < a.hidden ? *(const uint4*)(xrow[i] + k1) : make_uint4(0, 0, 0, 0);
             }
             __syncwarp();
-            const bf16* grow = a.gate + (i64)(k0 + lane) * a.E + j * 8;
+            const bf16* grow = (const bf16*)a.gate + (i64)(k0 + lane) * a.E + j * 8;
             if (a.E % 8 == 0) {
                 uint4 g[NB];
 #pragma unroll
@@ -293,7 +354,7 @@ template <bool ALL, int CW> __device__ __forceinline__ void find_expert(const Tc
 // with `tell`, `taken` and the weights in the workspace. `prefetch` is run by
 // the copying warp as soon as the loads of x and the gate are under way (before
 // them it would hold them up in the memory's queues).
-template <int R8, int CW, typename Prefetch>
+template <typename T, int R8, int CW, typename Prefetch>
 __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r, float* w_here, bool tell, Prefetch prefetch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cl = cg::this_cluster();
@@ -306,8 +367,9 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r,
     if (warp == CW) {
         asm volatile("bar.sync 1, %0;" ::"n"((CW + 1) * 32) : "memory");
         prefetch();
-    } else if (rows > 0 && warp * 32 < a.hidden) {
-        logits_tc<R8, CW>(a, t0, rows, room + CW * RT * MAX_E * 4, part, issued);
+    } else if (rows > 0 && warp * (64 / (int)sizeof(T)) < a.hidden) {
+        if constexpr (sizeof(T) == 4) logits_f32<R8, CW>(a, t0, rows, part, issued);
+        else logits_bf16<R8, CW>(a, t0, rows, room + CW * RT * MAX_E * 4, part, issued);
     } else {
         issued();
         for (int i = lane; i < RT * ep; i += 32) part[warp * RT * ep + i] = 0.f;
@@ -328,8 +390,8 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r,
         if (lane < copies) to[t] = taken;
         if (w_here || tell) {
             const bool in = taken >> lane & 1u;
-            float w = in ? __expf(l - top) : 0.f;
-            w = __fdividef(w, fmaxf(warp_sum(w), 1e-30f));
+            float w = in ? expf(l - top) : 0.f;
+            w /= fmaxf(warp_sum(w), 1e-30f);
             const int at = t * a.k + __popc(taken & ((1u << lane) - 1u));
             if (in && w_here) w_here[at] = w;
             if (tell) {
@@ -348,19 +410,21 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r,
 // weights and of as many token rows as the expert has, so that the usual few
 // tokens leave room for more stages.
 constexpr int MAX_STAGES = 8;
-template <bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
-    static constexpr int BN = BN_, BOX = BN < 64 ? BN : 64, THREADS = (CW + 1) * 32;
-    static constexpr int KG = CW * 16 / BN;  // groups of warps that share a tile's columns and split its k
-    static constexpr int W_BYTES = M * BK * BN * 2, RED_PITCH = BN + 4;  // bytes; floats
+template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
+    static constexpr int ES = sizeof(T), BN = BN_, BOX = BN < 128 / ES ? BN : 128 / ES, THREADS = (CW + 1) * 32;
+    // groups of warps that have the same columns (fp32: of one matrix) and split a tile's k
+    static constexpr int KG = ES == 4 ? CW / M : CW * 16 / BN;
+    static_assert(ES == 2 || BN == 32, "fp32: a lane to a column");
+    static constexpr int W_BYTES = M * BK * BN * ES, RED_PITCH = BN + 4;  // bytes; floats
     static constexpr int RED = M * NT * 8 * RED_PITCH;                   // floats of one group's sums
-    static constexpr int MIN_STAGES = ROOM / (W_BYTES + NT * 8 * XPITCH);
+    static constexpr int MIN_STAGES = ROOM / (W_BYTES + NT * 8 * XPITCH<T>);
     static constexpr int PRE = ALL ? (MIN_STAGES < 3 ? MIN_STAGES : 3) : 0;  // stages filled before routing
     static constexpr int SCRATCH = CW * (RT * MAX_E * 4 + (NT == 1 ? 8 : 4) * 512);
     static_assert(ROOM % 1024 == 0 && MIN_STAGES >= 2, "two stages at least");
     static_assert(KG * RED * 4 <= ROOM && (M == 1 && ALL ? 0 : PRE * W_BYTES + SCRATCH) <= ROOM,
                   "the parts, and routing beside the first stages, lie in the ring");
     static_assert(1024 + ROOM + 2 * MAX_STAGES * 8 + MAX_T * (8 + 4 * MAX_E) <= SMEM_MAX, "smem()'s largest");
-    static size_t smem(int T, int k) { return 1024 + ROOM + 2 * MAX_STAGES * 8 + routes_bytes(T, k); }
+    static size_t smem(int tokens, int k) { return 1024 + ROOM + 2 * MAX_STAGES * 8 + routes_bytes(tokens, k); }
 
     char* ring;
     uint64_t *full, *empty;
@@ -402,7 +466,7 @@ template <bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
         for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int c = 0; c < BN; c += BOX)
-                tc::tma_load_3d(at + (m * BN + c) * BK * 2, w[m], col0 + c, r0 + it * BK, expert, &full[st]);
+                tc::tma_load_3d(at + (m * BN + c) * BK * ES, w[m], col0 + c, r0 + it * BK, expert, &full[st]);
     }
     // An expert that no token takes: let what was fetched land, then leave.
     __device__ __forceinline__ void drain(const TcArgs& a) const {
@@ -417,29 +481,35 @@ template <bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
 // Rows [r0, r1) of the expert's matrices times the same columns of `rows`
 // (row index `idx`, row length `len`), left in shared memory: sum(m, token
 // index, column in the tile).
-template <bool ALL, int M, int NT, int BN, int CW, int ROOM, typename Wait>
-__device__ __forceinline__ void product(const Tc<ALL, M, NT, BN, CW, ROOM>& s, const TcArgs& a, const Routes& r, const short* idx,
-                                        const bf16* rows, int len, Wait wait) {
-    using S = Tc<ALL, M, NT, BN, CW, ROOM>;
+template <typename T, bool ALL, int M, int NT, int BN, int CW, int ROOM, typename Wait>
+__device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s, const TcArgs& a, const Routes& r, const short* idx,
+                                        const T* rows, int len, Wait wait) {
+    using S = Tc<T, ALL, M, NT, BN, CW, ROOM>;
+    using namespace tc::pairs;
+    constexpr bool F32 = sizeof(T) == 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int iters = s.iters, nte = (r.n + 7) / 8, xbytes = nte * 8 * XPITCH;
+    const int iters = s.iters, nte = (r.n + 7) / 8, xbytes = nte * 8 * XPITCH<T>;
     const int stages = min(MAX_STAGES, ROOM / (S::W_BYTES + xbytes));
     char* const xring = s.ring + stages * S::W_BYTES;
-    float acc[M][NT][4];
+    float acc[F32 ? 1 : M][NT][4];  // bf16: the fragments
+    f2 sum[F32 ? NT * 8 : 1];       // fp32: a token's even and odd k
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+    for (int m = 0; m < (F32 ? 1 : M); ++m)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int u = 0; u < 4; ++u) acc[m][j][u] = 0.f;
+#pragma unroll
+    for (int t = 0; t < (F32 ? NT * 8 : 1); ++t) sum[t] = pack2(0.f, 0.f);
     if (warp == CW) {
         auto tokens = [&](int it, int st) {
+            constexpr int P = BK / PIECE<T>;  // 16-byte pieces of a row
             const uint32_t at = tc::smem_u32(xring + st * xbytes);
-            const int k0 = s.r0 + it * BK, chunks = (min(s.r1, k0 + BK) - k0) >> 3;  // of 8 k
-            for (int i = lane; i < r.n * 8; i += 32) {
-                const int row = i >> 3, c = i & 7;
-                const bool on = c < chunks;
-                tc::cp_async16(at + row * XPITCH + c * 16, rows + (i64)idx[row] * len + (on ? k0 + c * 8 : 0), on);
+            const int k0 = s.r0 + it * BK, pieces = (min(s.r1, k0 + BK) - k0) / PIECE<T>;
+            for (int i = lane; i < r.n * P; i += 32) {
+                const int row = i / P, c = i % P;
+                const bool on = c < pieces;
+                tc::cp_async16(at + row * XPITCH<T> + c * 16, rows + (i64)idx[row] * len + (on ? k0 + c * PIECE<T> : 0), on);
             }
             tc::cp_async_arrive(&s.full[st]);
         };
@@ -454,6 +524,35 @@ __device__ __forceinline__ void product(const Tc<ALL, M, NT, BN, CW, ROOM>& s, c
             if (lane == 0) s.weights(it, st, r.expert);
             __syncwarp();
             tokens(it, st);
+            if (++st == stages) st = 0, ph ^= 1;
+        }
+    } else if constexpr (F32) {
+        wait();
+        constexpr int R = BK / S::KG;  // rows of a tile that a warp takes
+        const int m = warp % M, kg = warp / M;
+        for (int it = 0, st = 0, ph = 0; it < iters; ++it) {
+            const int kk = min(BK, s.r1 - s.r0 - it * BK);
+            tc::mbar_wait(&s.full[st], ph, a.status, 4, 4000000000ll, false);
+            const float* wt = (const float*)(s.ring + st * S::W_BYTES) + m * BK * BN + lane;
+            const char* xt = xring + st * xbytes;
+#pragma unroll
+            for (int q = 0; q < R; q += 4) {
+                const int k = kg * R + q;
+                if (k >= kk) break;  // kk is a multiple of 4
+                const f2 w01 = pack2(wt[k * BN], wt[(k + 1) * BN]), w23 = pack2(wt[(k + 2) * BN], wt[(k + 3) * BN]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if (j >= nte) break;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const ulonglong2 x = *(const ulonglong2*)(xt + (j * 8 + u) * XPITCH<T> + k * 4);
+                        sum[j * 8 + u] = fma2(w01, x.x, sum[j * 8 + u]);
+                        sum[j * 8 + u] = fma2(w23, x.y, sum[j * 8 + u]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.empty[st]);
             if (++st == stages) st = 0, ph ^= 1;
         }
     } else {
@@ -483,7 +582,7 @@ __device__ __forceinline__ void product(const Tc<ALL, M, NT, BN, CW, ROOM>& s, c
                 for (int j = 0; j < NT; ++j) {
                     if (j >= nte) break;
                     uint32_t b[4];
-                    tc::ldsm4(b, xb + (j * 8 + k8) * XPITCH + (k0 / 8 + (lane >> 3)) * 16);
+                    tc::ldsm4(b, xb + (j * 8 + k8) * XPITCH<T> + (k0 / 8 + (lane >> 3)) * 16);
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
                         tc::mma16816(acc[m][j], wa[m][0], b[0], b[1]);
@@ -497,7 +596,13 @@ __device__ __forceinline__ void product(const Tc<ALL, M, NT, BN, CW, ROOM>& s, c
         }
     }
     __syncthreads();  // every tile of the ring has landed and been read
-    if (warp < CW) {
+    if (warp == CW) return;
+    if constexpr (F32) {
+        float* red = (float*)s.ring + warp / M * S::RED + warp % M * NT * 8 * S::RED_PITCH + lane;
+#pragma unroll
+        for (int t = 0; t < NT * 8; ++t)
+            if (t < r.n) red[t * S::RED_PITCH] = sum2(sum[t]);
+    } else {
         const int wm = warp % (BN / 16), kg = warp / (BN / 16);
         float* red = (float*)s.ring + kg * S::RED + wm * 16 + (lane >> 2) + (lane & 3) * 2 * S::RED_PITCH;
 #pragma unroll
@@ -526,18 +631,18 @@ template <typename S, int M, int NT> __device__ __forceinline__ void add_sums(co
         }
 }
 
-template <bool ALL, int NT, int BN, int CW, int ROOM, int PER_SM>
+template <typename T, bool ALL, int NT, int BN, int CW, int ROOM, int PER_SM>
 __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     k_up_tc(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap w1, const __grid_constant__ CUtensorMap w3) {
     extern __shared__ char raw[];
     tc::launch_dependents();  // the second kernel may take the SMs' free places and fetch w2
     Routes r;
-    using S = Tc<ALL, 2, NT, BN, CW, ROOM>;
+    using S = Tc<T, ALL, 2, NT, BN, CW, ROOM>;
     const S s(a, raw, r, &w1, &w3, a.up_run, a.hidden, a.mid);
     const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
     if (first)
-        for (int i = threadIdx.x; i < (a.hidden + 63) / 64; i += S::THREADS) a.count[i] = 0u;
-    route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring + S::PRE * S::W_BYTES, r, nullptr,
+        for (int i = threadIdx.x; i < (a.hidden + 31) / 32; i += S::THREADS) a.count[i] = 0u;
+    route_tc<T, NT == 1 ? 1 : 2, CW>(a, s.ring + S::PRE * S::W_BYTES, r, nullptr,
                                   ALL && blockIdx.x < cg::this_cluster().dim_blocks().x && blockIdx.z == 0, [&] { s.prefetch(); });
     find_expert<ALL, CW>(a, blockIdx.z, r);
     if (r.n == 0) {  // the whole cluster: it shares its slot
@@ -545,7 +650,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         return;
     }
     __syncthreads();
-    product(s, a, r, r.tok, a.x, a.hidden, [] {});
+    product(s, a, r, r.tok, (const T*)a.x, a.hidden, [] {});
     // the runs of a tile add their sums up in rank order, each a share of the tile
     cg::cluster_group cl = cg::this_cluster();
     const int runs = gridDim.y, run = blockIdx.y, cx = (int)cl.dim_blocks().x, ix = (int)cl.block_index().x;
@@ -561,21 +666,21 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         const float* u = (const float*)&v[0];
         const float* g = (const float*)&v[1];
         float h[4];
-        // held in bf16, the type that the second product multiplies in
+        // held in the type that the second product multiplies in
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = u[j] / (1.f + __expf(-u[j])) * g[j];
-        stv<bf16, 4>(a.h + (i64)r.pair[t] * a.mid + s.col0 + c, h);
+        for (int j = 0; j < 4; ++j) h[j] = u[j] / (1.f + (sizeof(T) == 4 ? expf(-u[j]) : __expf(-u[j]))) * g[j];
+        stv<T, 4>((T*)a.h + (i64)r.pair[t] * a.mid + s.col0 + c, h);
     }
     if (runs > 1) cl.sync();  // no CTA leaves while another reads its sums
 }
 
-template <bool ALL, int NT, int BN, int CW, int ROOM, int PER_SM>
+template <typename T, bool ALL, int NT, int BN, int CW, int ROOM, int PER_SM>
 __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     k_down_tc(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap w2) {
     extern __shared__ char raw[];
     __shared__ bool last;
     Routes r;
-    using S = Tc<ALL, 1, NT, BN, CW, ROOM>;
+    using S = Tc<T, ALL, 1, NT, BN, CW, ROOM>;
     const S s(a, raw, r, &w2, &w2, a.down_run, a.mid, a.hidden);
     if (ALL) {
         s.prefetch();
@@ -583,7 +688,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         for (int i = threadIdx.x; i < a.T * (a.k + 1); i += S::THREADS) r.taken[i] = __ldcg(a.taken + i);
         __syncthreads();
     } else {
-        route_tc<NT == 1 ? 1 : 2, CW>(a, s.ring, r, r.w, false, [] {});
+        route_tc<T, NT == 1 ? 1 : 2, CW>(a, s.ring, r, r.w, false, [] {});
     }
     find_expert<ALL, CW>(a, blockIdx.z, r);
     if (r.n == 0) {
@@ -592,7 +697,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     }
     __syncthreads();
     const int col0 = s.col0;
-    product(s, a, r, r.pair, a.h, a.mid, [] { if (!ALL) tc::grid_dependency_wait(); });
+    product(s, a, r, r.pair, (const T*)a.h, a.mid, [] { if (!ALL) tc::grid_dependency_wait(); });
     __syncthreads();
     const i64 run_size = (i64)a.T * a.k * a.hidden;
 #pragma unroll 1
@@ -648,7 +753,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         for (int i = 0; i < AT_ONCE; ++i) {
             const int t = tb + i * (S::THREADS / Q);
             const float o[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-            if (t < a.T) stv<bf16, 4>(a.y + (i64)t * a.hidden + c, o);
+            if (t < a.T) stv<T, 4>((T*)a.y + (i64)t * a.hidden + c, o);
         }
     }
 }
@@ -718,14 +823,21 @@ template <bool ALL_, int NT_, int BU_, int CU_, int RU_, int PU_, int BD_, int C
 };
 
 // f(Shape) for a problem.
-template <typename F> static void with_shape(Context* c, i64 T, i64 mid, i64 slots, F f) {
-    const bool thin = (i64)cdiv(mid, 32) * slots <= (i64)c->sm_count * 4;
-    if (T <= 8 && thin) f(Shape<false, 1, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
-    else if (T <= 8) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
-    else if (T <= 16 && thin) f(Shape<false, 2, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
-    else if (T <= 16) f(Shape<false, 2, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
-    else if (T <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
-    else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+template <typename T, typename F> static void with_shape(Context* c, i64 T_, i64 mid, i64 slots, F f) {
+    if constexpr (sizeof(T) == 4) {
+        if (T_ <= 8) f(Shape<false, 1, 32, 8, 60 * K, 3, 32, 8, 60 * K, 3>());
+        else if (T_ <= 16) f(Shape<false, 2, 32, 8, 60 * K, 3, 32, 8, 60 * K, 3>());
+        else if (T_ <= 32) f(Shape<true, 4, 32, 8, 104 * K, 2, 32, 8, 104 * K, 2>());
+        else f(Shape<true, 8, 32, 8, 120 * K, 1, 32, 8, 120 * K, 1>());
+    } else {
+        const bool thin = (i64)cdiv(mid, 32) * slots <= (i64)c->sm_count * 4;
+        if (T_ <= 8 && thin) f(Shape<false, 1, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
+        else if (T_ <= 8) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
+        else if (T_ <= 16 && thin) f(Shape<false, 2, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
+        else if (T_ <= 16) f(Shape<false, 2, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
+        else if (T_ <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+        else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+    }
 }
 
 // Where things lie in the workspace of the tensor-core kernels.
@@ -733,35 +845,38 @@ struct Layout {
     size_t yp, count, taken, bytes;
 };
 static int slots_of(i64 T, i64 E, i64 k) { return (int)(T > 16 ? E : std::min(E, T * k)); }
-static Layout layout(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k) {
+template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k) {
     Layout l{};
     const int slots = slots_of(T, E, k);
-    with_shape(c, T, mid, slots, [&](auto shape) {
+    with_shape<Ty>(c, T, mid, slots, [&](auto shape) {
         using P = decltype(shape);
         const Plan d = plan(c, slots, (int)T, false, (int)mid, (int)hidden, P::BD, P::PD);
-        l.yp = align256((size_t)T * k * mid * 2);
+        l.yp = align256((size_t)T * k * mid * sizeof(Ty));
         l.count = l.yp + align256((size_t)d.grid.y * T * k * hidden * 4);
-        l.taken = l.count + align256((size_t)cdiv(hidden, 64) * 4);
+        l.taken = l.count + align256((size_t)cdiv(hidden, 32) * 4);
         l.bytes = l.taken + align256((size_t)T * (k + 1) * 4);
     });
     return l;
 }
 
-static void run_tc(Context* c, TcArgs a, const void* w1, const void* w3, const void* w2) {
+template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, const void* w3, const void* w2) {
     const int slots = slots_of(a.T, a.E, a.k);
-    with_shape(c, a.T, a.mid, slots, [&](auto shape) {
+    with_shape<T>(c, a.T, a.mid, slots, [&](auto shape) {
         using P = decltype(shape);
-        const CUtensorMap m1 = tma_map_stack(w1, a.E, a.hidden, a.mid, CATNN_BF16, std::min(64, P::BU), BK);
-        const CUtensorMap m3 = tma_map_stack(w3, a.E, a.hidden, a.mid, CATNN_BF16, std::min(64, P::BU), BK);
-        const CUtensorMap m2 = tma_map_stack(w2, a.E, a.mid, a.hidden, CATNN_BF16, std::min(64, P::BD), BK);
+        using U = Tc<T, P::ALL, 2, P::NT, P::BU, P::CU, P::RU>;
+        using D = Tc<T, P::ALL, 1, P::NT, P::BD, P::CD, P::RD>;
+        const int dt = sizeof(T) == 4 ? CATNN_F32 : CATNN_BF16;
+        const CUtensorMap m1 = tma_map_stack(w1, a.E, a.hidden, a.mid, dt, U::BOX, BK);
+        const CUtensorMap m3 = tma_map_stack(w3, a.E, a.hidden, a.mid, dt, U::BOX, BK);
+        const CUtensorMap m2 = tma_map_stack(w2, a.E, a.mid, a.hidden, dt, D::BOX, BK);
         const Plan u = plan(c, slots, a.T, true, a.hidden, a.mid, P::BU, P::PU);
         const Plan d = plan(c, slots, a.T, false, a.mid, a.hidden, P::BD, P::PD);
         a.up_run = u.run;
         a.down_run = d.run;
-        launch(c, k_up_tc<P::ALL, P::NT, P::BU, P::CU, P::RU, P::PU>, (P::CU + 1) * 32, u.grid, u.cluster,
-               Tc<P::ALL, 2, P::NT, P::BU, P::CU, P::RU>::smem(a.T, a.k), false, a, m1, m3);
-        launch(c, k_down_tc<P::ALL, P::NT, P::BD, P::CD, P::RD, P::PD>, (P::CD + 1) * 32, d.grid, d.cluster,
-               Tc<P::ALL, 1, P::NT, P::BD, P::CD, P::RD>::smem(a.T, a.k), true, a, m2);
+        launch(c, k_up_tc<T, P::ALL, P::NT, P::BU, P::CU, P::RU, P::PU>, U::THREADS, u.grid, u.cluster, U::smem(a.T, a.k), false, a,
+               m1, m3);
+        launch(c, k_down_tc<T, P::ALL, P::NT, P::BD, P::CD, P::RD, P::PD>, D::THREADS, d.grid, d.cluster, D::smem(a.T, a.k), true, a,
+               m2);
     });
 }
 
@@ -773,21 +888,30 @@ using namespace few;
 size_t moe_few_workspace(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k, int dtype) {
     if (T == 0) return 0;
     const size_t plain = (size_t)T * k * mid * sizeof(float);
-    return dtype == CATNN_BF16 ? std::max(plain, layout(c, T, hidden, mid, E, k).bytes) : plain;
+    return std::max(plain, dtype == CATNN_BF16 ? layout<bf16>(c, T, hidden, mid, E, k).bytes
+                                               : layout<float>(c, T, hidden, mid, E, k).bytes);
+}
+
+template <typename Ty>
+static void moe_few_tc(Context* c, const void* x, const void* gate, const void* w1, const void* w3, const void* w2, void* y, i64 T,
+                       i64 hidden, i64 mid, i64 E, i64 k, void* work) {
+    const Layout l = layout<Ty>(c, T, hidden, mid, E, k);
+    char* at = (char*)work;
+    run_tc<Ty>(c,
+               {x, gate, work, y, (float*)(at + l.yp), (unsigned*)(at + l.taken), (unsigned*)(at + l.count), c->status, (int)T,
+                (int)hidden, (int)mid, (int)E, (int)k, 0, 0},
+               w1, w3, w2);
 }
 
 void moe_few(Context* c, const void* x, const void* gate, const void* w1, const void* w3, const void* w2, void* y, i64 T,
              i64 hidden, i64 mid, i64 E, i64 k, int dtype, void* work) {
     if (T == 0) return;
     const auto al = [](const void* p) { return aligned_to(p, 16); };
-    if (dtype == CATNN_BF16 && hidden % 8 == 0 && mid % 8 == 0 && hidden >= BK && mid >= BK && al(x) && al(gate) && al(w1) &&
-        al(w3) && al(w2) && al(y)) {
-        const Layout l = layout(c, T, hidden, mid, E, k);
-        char* at = (char*)work;
-        run_tc(c,
-               {(const bf16*)x, (const bf16*)gate, (bf16*)work, (bf16*)y, (float*)(at + l.yp), (unsigned*)(at + l.taken),
-                (unsigned*)(at + l.count), c->status, (int)T, (int)hidden, (int)mid, (int)E, (int)k, 0, 0},
-               w1, w3, w2);
+    const int piece = dtype == CATNN_BF16 ? 8 : 4;
+    if (hidden % piece == 0 && mid % piece == 0 && hidden >= BK && mid >= BK && al(x) && al(gate) && al(w1) && al(w3) && al(w2) &&
+        al(y)) {
+        if (dtype == CATNN_BF16) moe_few_tc<bf16>(c, x, gate, w1, w3, w2, y, T, hidden, mid, E, k, work);
+        else moe_few_tc<float>(c, x, gate, w1, w3, w2, y, T, hidden, mid, E, k, work);
         return;
     }
     Args a{x, gate, w1, w3, w2, y, (float*)work, (int)T, (int)hidden, (int)mid, (int)E, (int)k};

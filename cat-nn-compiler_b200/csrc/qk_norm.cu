@@ -70,31 +70,7 @@ template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 // What bounds these kernels next to HBM is the number of instructions, so a
 // lane's values are taken two pairs at a time: X0 = the first elements of
 // pairs i and i + 1, X1 = their second elements.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack2(float a, float b) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 split2(f2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float sum2(f2 v) {
-    const float2 s = split2(v);
-    return s.x + s.y;
-}
+using namespace tc::pairs;
 
 // 16 bytes as packed pairs, and back.
 template <typename T> constexpr int NP = VEC<T> / 4;

@@ -715,46 +715,49 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     __syncthreads();
     if (!last) return;
     __threadfence();
-    // four tokens at a time, so that their loads are in flight together
-    constexpr int Q = BN / 4, AT_ONCE = 4;
-    const int c = col0 + threadIdx.x % Q * 4;
-    if (c >= a.hidden) return;
-#pragma unroll 1
-    for (int tb = threadIdx.x / Q; tb < a.T; tb += S::THREADS / Q * AT_ONCE) {
-        float4 y[AT_ONCE];
+    // A thread's terms (its tokens, their experts, the runs) in one row, eight of them on their way at a time.
+    constexpr int Q = BN / 4, TEAMS = S::THREADS / Q, FLIGHT = 8;
+    const int c = col0 + threadIdx.x % Q * 4, team = threadIdx.x / Q, runs = gridDim.y;
+    if (c >= a.hidden || team >= TEAMS || team >= a.T) return;
+    int left = ((a.T - 1 - team) / TEAMS + 1) * a.k * runs;
+    int lt = team, lj = 0, lq = 0, t = team, j = 0, q = 0;  // of the next term to load, to add
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), y = v;
+    while (left > 0) {
+        float4 u[FLIGHT];
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int j = 0; j < a.k; ++j) {
-            float4 v[AT_ONCE];
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-            for (int q = 0; q < (int)gridDim.y; ++q)
-#pragma unroll
-                for (int i = 0; i < AT_ONCE; ++i) {
-                    const int t = min(tb + i * (S::THREADS / Q), a.T - 1);
-                    const float4 u = __ldcg((const float4*)(a.yp + q * run_size + ((i64)t * a.k + j) * a.hidden + c));
-                    v[i].x += u.x;
-                    v[i].y += u.y;
-                    v[i].z += u.z;
-                    v[i].w += u.w;
-                }
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) {
-                const float w = r.w[min(tb + i * (S::THREADS / Q), a.T - 1) * a.k + j];
-                y[i].x = fmaf(w, v[i].x, y[i].x);
-                y[i].y = fmaf(w, v[i].y, y[i].y);
-                y[i].z = fmaf(w, v[i].z, y[i].z);
-                y[i].w = fmaf(w, v[i].w, y[i].w);
+        for (int i = 0; i < FLIGHT; ++i) {
+            if (i >= left) break;
+            u[i] = __ldcg((const float4*)(a.yp + lq * run_size + ((i64)lt * a.k + lj) * a.hidden + c));
+            if (++lq == runs) {
+                lq = 0;
+                if (++lj == a.k) lj = 0, lt += TEAMS;
             }
         }
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-            const int t = tb + i * (S::THREADS / Q);
-            const float o[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-            if (t < a.T) stv<T, 4>((T*)a.y + (i64)t * a.hidden + c, o);
+        for (int i = 0; i < FLIGHT; ++i) {
+            if (i >= left) break;
+            v.x += u[i].x;
+            v.y += u[i].y;
+            v.z += u[i].z;
+            v.w += u[i].w;
+            if (++q == runs) {
+                const float w = r.w[t * a.k + j];
+                y.x = fmaf(w, v.x, y.x);
+                y.y = fmaf(w, v.y, y.y);
+                y.z = fmaf(w, v.z, y.z);
+                y.w = fmaf(w, v.w, y.w);
+                v = make_float4(0.f, 0.f, 0.f, 0.f);
+                q = 0;
+                if (++j == a.k) {
+                    const float o[4] = {y.x, y.y, y.z, y.w};
+                    stv<T, 4>((T*)a.y + (i64)t * a.hidden + c, o);
+                    y = v;
+                    j = 0;
+                    t += TEAMS;
+                }
+            }
         }
+        left -= FLIGHT;
     }
 }
 

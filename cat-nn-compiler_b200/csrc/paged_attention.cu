@@ -28,7 +28,6 @@ namespace paged {
 
 constexpr int MAX_HD = 128;
 constexpr int TK = 32;         // positions of a tile: one a lane
-constexpr int MIN_TILES = 4;   // of a warp, where there are few: fewer would make the join dearer than the reading
 constexpr int MAX_CHUNKS = 512;
 
 struct Args {
@@ -104,7 +103,7 @@ template <int W> __device__ __forceinline__ Count count_tiles(const Args& a, int
         c.own = 0;
         c.total = warp_sum_int(s);
     }
-    c.workers = max(1, min(a.workers, (c.total + MIN_TILES - 1) / MIN_TILES));
+    c.workers = max(1, min(a.workers, c.total));
     c.each = c.total / c.workers;
     c.more = c.total - c.each * c.workers;
     return c;
@@ -714,16 +713,20 @@ __global__ void __launch_bounds__(WARPS * 32) k_paged_any(const __grid_constant_
 }
 
 // ------------------------------------------------------------ launchers
-// Warps and CTAs of the streaming kernels by type and head size: as many
-// warps as the SM's shared memory holds rings for (up to eight).
+// Warps and CTAs of the streaming kernels by type and head size: enough rings
+// of two stages to keep the memory busy (a third stage, or as many warps more,
+// made no call faster), and for fp32, whose warps have more to compute, as
+// many as the SM's shared memory holds.
 struct Fill {
     int warps, per_sm, rows;  // warps of a CTA, CTAs an SM, query heads of a row tile
 };
+static constexpr int mma_warps(int hd) { return hd <= 64 ? 4 : 5; }
+static constexpr int fma_warps(int hd) { return hd <= 64 ? 6 : hd <= 96 ? 4 : 3; }
 static Fill fill_of(int dtype, int hd, int group) {
-    if (dtype == CATNN_BF16) return hd <= 64 ? Fill{4, 2, group <= 8 ? 8 : 16} : Fill{4, 1, group <= 8 ? 8 : 16};
-    const int rows = group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
-    return Fill{hd <= 96 ? 4 : 3, 1, rows};
+    if (dtype == CATNN_BF16) return Fill{mma_warps(hd), hd <= 64 ? 2 : 1, group <= 8 ? 8 : 16};
+    return Fill{fma_warps(hd), 1, group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8};
 }
+constexpr int STAGES = 2;
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -754,17 +757,26 @@ template <typename Kern> static void launch(Context* c, Kern k, int grid, int th
     launched(c);
 }
 
-template <int HDP, int R8, int S> static void run_mma(Context* c, const Args& a, const Fill& f) {
-    launch(c, k_paged_mma<HDP, R8, S, 4>, c->sm_count * f.per_sm, 128, 4 * Ring<bf16, HDP, S>::BYTES, a);
+template <int HDP, int R8> static void run_mma(Context* c, const Args& a, const Fill& f) {
+    constexpr int W = mma_warps(HDP);
+    launch(c, k_paged_mma<HDP, R8, STAGES, W>, c->sm_count * f.per_sm, W * 32, W * Ring<bf16, HDP, STAGES>::BYTES, a);
 }
-template <int HDP, int G, int S, int W> static void run_fma(Context* c, const Args& a, const Fill& f) {
-    launch(c, k_paged_fma<HDP, G, S, W>, c->sm_count * f.per_sm, W * 32, W * (Ring<float, HDP, S>::BYTES + G * (HDP + TK) * 4), a);
+template <int HDP, int G> static void run_fma(Context* c, const Args& a, const Fill& f) {
+    constexpr int W = fma_warps(HDP), BYTES = W * (Ring<float, HDP, STAGES>::BYTES + G * (HDP + TK) * 4);
+    static_assert(BYTES + MAX_CHUNKS * 4 <= 232448, "shared memory of a CTA");
+    launch(c, k_paged_fma<HDP, G, STAGES, W>, c->sm_count * f.per_sm, W * 32, BYTES, a);
+}
+template <int R8> static void run_mma_hd(Context* c, const Args& a, const Fill& f) {
+    if (a.hd <= 32) run_mma<32, R8>(c, a, f);
+    else if (a.hd <= 64) run_mma<64, R8>(c, a, f);
+    else if (a.hd <= 96) run_mma<96, R8>(c, a, f);
+    else run_mma<128, R8>(c, a, f);
 }
 template <int G> static void run_fma_hd(Context* c, const Args& a, const Fill& f) {
-    if (a.hd <= 32) run_fma<32, G, 3, 4>(c, a, f);
-    else if (a.hd <= 64) run_fma<64, G, 3, 4>(c, a, f);
-    else if (a.hd <= 96) run_fma<96, G, 2, 4>(c, a, f);
-    else run_fma<128, G, 2, 3>(c, a, f);
+    if (a.hd <= 32) run_fma<32, G>(c, a, f);
+    else if (a.hd <= 64) run_fma<64, G>(c, a, f);
+    else if (a.hd <= 96) run_fma<96, G>(c, a, f);
+    else run_fma<128, G>(c, a, f);
 }
 
 }  // namespace paged
@@ -796,11 +808,8 @@ void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, co
                 "paged_attention: the table's positions times the heads pass 2^31 tiles of 32");
     const Fill f = fill_of(dtype, (int)hd, (int)(h / hkv));
     if (dtype == CATNN_BF16) {
-        const bool eight = f.rows == 8;
-        if (hd <= 32) eight ? run_mma<32, 1, 3>(c, a, f) : run_mma<32, 2, 3>(c, a, f);
-        else if (hd <= 64) eight ? run_mma<64, 1, 3>(c, a, f) : run_mma<64, 2, 3>(c, a, f);
-        else if (hd <= 96) eight ? run_mma<96, 1, 3>(c, a, f) : run_mma<96, 2, 3>(c, a, f);
-        else eight ? run_mma<128, 1, 3>(c, a, f) : run_mma<128, 2, 3>(c, a, f);
+        if (f.rows == 8) run_mma_hd<1>(c, a, f);
+        else run_mma_hd<2>(c, a, f);
     } else {
         if (f.rows == 1) run_fma_hd<1>(c, a, f);
         else if (f.rows == 2) run_fma_hd<2>(c, a, f);

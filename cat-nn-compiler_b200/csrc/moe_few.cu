@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(THREADS) k_down_any(const __grid_constant__ Ar
 // swizzled tiles. The runs of one tile lie in one cluster, which adds its
 // parts up through distributed shared memory in rank order.
 //
-// Of up to 16 tokens the experts that any token takes are found first, by
-// every CTA of both kernels for itself (ALL = false): a slot of the grid is the
-// slot-th of them. Of more tokens (nearly) every expert has some: a slot is an
+// Where few experts are chosen, they are found first, by every CTA of both
+// kernels for itself (ALL = false): a slot of the grid is the slot-th of them.
+// With more choices (nearly) every expert has some token: a slot is an
 // expert, whose first tiles are fetched while the first kernel routes, and
 // the second kernel, whose first tiles are fetched beside the first's last,
 // reads what the first found (ALL = true).
@@ -825,20 +825,29 @@ template <bool ALL_, int NT_, int BU_, int CU_, int RU_, int PU_, int BD_, int C
     static constexpr int NT = NT_, BU = BU_, CU = CU_, RU = RU_, PU = PU_, BD = BD_, CD = CD_, RD = RD_, PD = PD_;
 };
 
+// Whether a slot of the grid is an expert, or the chosen experts are found
+// before anything is fetched. With few choices most experts' tiles would be
+// fetched in vain. Hidden 1024, mid 3584, 8 experts, top 2: at 4 tokens 31.4 us
+// found first against 29.8, at 16 tokens 41.4 against 36.4; 8 tokens' top 4 of 32
+// (hidden 512, mid 1000) 38.7 against 26.2. fp32, whose CTAs are many, gains
+// nothing from it at 16 tokens (111 us either way).
+template <typename T> static bool slot_is_expert(i64 tokens, i64 E, i64 k) {
+    return sizeof(T) == 4 ? tokens > 16 : tokens > 8 || tokens * k >= E;
+}
+
 // f(Shape) for a problem.
-template <typename T, typename F> static void with_shape(Context* c, i64 T_, i64 mid, i64 slots, F f) {
+template <typename T, typename F> static void with_shape(Context* c, i64 tokens, i64 mid, i64 E, i64 k, F f) {
+    const bool all = slot_is_expert<T>(tokens, E, k);
     if constexpr (sizeof(T) == 4) {
-        if (T_ <= 8) f(Shape<false, 1, 32, 8, 60 * K, 3, 32, 8, 60 * K, 3>());
-        else if (T_ <= 16) f(Shape<false, 2, 32, 8, 60 * K, 3, 32, 8, 60 * K, 3>());
-        else if (T_ <= 32) f(Shape<true, 4, 32, 8, 104 * K, 2, 32, 8, 104 * K, 2>());
+        if (tokens <= 8) f(Shape<false, 1, 32, 4, 52 * K, 3, 32, 4, 52 * K, 3>());
+        else if (!all) f(Shape<false, 2, 32, 4, 52 * K, 4, 32, 4, 52 * K, 4>());
+        else if (tokens <= 32) f(Shape<true, 4, 32, 8, 104 * K, 2, 32, 8, 104 * K, 2>());
         else f(Shape<true, 8, 32, 8, 120 * K, 1, 32, 8, 120 * K, 1>());
     } else {
-        const bool thin = (i64)cdiv(mid, 32) * slots <= (i64)c->sm_count * 4;
-        if (T_ <= 8 && thin) f(Shape<false, 1, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
-        else if (T_ <= 8) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
-        else if (T_ <= 16 && thin) f(Shape<false, 2, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
-        else if (T_ <= 16) f(Shape<false, 2, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
-        else if (T_ <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+        // thin tiles, where they fit on the SMs at once, need no cluster to cut their rows
+        if (!all && (i64)cdiv(mid, 32) * tokens * k <= (i64)c->sm_count * 4) f(Shape<false, 1, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
+        else if (!all) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
+        else if (tokens <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
         else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
     }
 }
@@ -847,11 +856,13 @@ template <typename T, typename F> static void with_shape(Context* c, i64 T_, i64
 struct Layout {
     size_t yp, count, taken, bytes;
 };
-static int slots_of(i64 T, i64 E, i64 k) { return (int)(T > 16 ? E : std::min(E, T * k)); }
+template <typename T> static int slots_of(i64 tokens, i64 E, i64 k) {
+    return (int)(slot_is_expert<T>(tokens, E, k) ? E : std::min(E, tokens * k));
+}
 template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k) {
     Layout l{};
-    const int slots = slots_of(T, E, k);
-    with_shape<Ty>(c, T, mid, slots, [&](auto shape) {
+    const int slots = slots_of<Ty>(T, E, k);
+    with_shape<Ty>(c, T, mid, E, k, [&](auto shape) {
         using P = decltype(shape);
         const Plan d = plan(c, slots, (int)T, false, (int)mid, (int)hidden, P::BD, P::PD);
         l.yp = align256((size_t)T * k * mid * sizeof(Ty));
@@ -863,8 +874,8 @@ template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 m
 }
 
 template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, const void* w3, const void* w2) {
-    const int slots = slots_of(a.T, a.E, a.k);
-    with_shape<T>(c, a.T, a.mid, slots, [&](auto shape) {
+    const int slots = slots_of<T>(a.T, a.E, a.k);
+    with_shape<T>(c, a.T, a.mid, a.E, a.k, [&](auto shape) {
         using P = decltype(shape);
         using U = Tc<T, P::ALL, 2, P::NT, P::BU, P::CU, P::RU>;
         using D = Tc<T, P::ALL, 1, P::NT, P::BD, P::CD, P::RD>;

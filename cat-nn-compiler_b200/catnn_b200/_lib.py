@@ -139,7 +139,7 @@ def last_error():
 
 def call(name, *args):
     """Call an entry point and raise the matching CatError on failure."""
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != 0:
         raise_for(rc, f"{name}: {last_error()}")
     return rc

@@ -550,9 +550,9 @@ def _rows(t, what):
     dense and whose tokens evenly spaced: a tensor of its own, or a column
     block of the rows that one QKV product writes."""
     *lead, heads, hd = t.shape
-    *st, per_head, per_value = t.stride()
-    if t.numel() == 0:
+    if t.is_contiguous() or t.numel() == 0:
         return heads * hd
+    *st, per_head, per_value = t.stride()
     if (hd > 1 and per_value != 1) or (heads > 1 and per_head != hd):
         raise InvalidArgument(f"{what}: a token's heads must be dense")
     token, span = heads * hd, None  # span: stride of the next outer dimension that is evenly spaced
@@ -566,6 +566,10 @@ def _rows(t, what):
             raise InvalidArgument(f"{what}: tokens must be evenly spaced")
         span = step * n
     return token
+
+
+def _dense_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _i32(t, what):
@@ -588,7 +592,8 @@ def _qk(q, k, what):
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]:
         raise ShapeMismatch(f"{what}: q {tuple(qs)}, k {tuple(ks)}")
-    _same(q, k)
+    if q.dtype != k.dtype:
+        _same(q, k)
     b, s, h, hd = qs
     return b, s, h, ks[2], hd
 
@@ -609,7 +614,7 @@ def qk_norm_rope(q, k, wq, wk, theta, eps=1e-5, positions=None):
     b, s, h, hkv, hd = _qk(q, k, "qk_norm_rope")
     pos = _positions(positions, b, s, "qk_norm_rope")
     ctx = _on(q, k, wq, wk, positions)
-    qo, ko = q.new_empty((b, s, h, hd)), k.new_empty((b, s, hkv, hd))
+    qo, ko = _dense_like(q), _dense_like(k)
     _lib.call("catnn_qk_norm_rope_fwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
               _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, qo.data_ptr(), ko.data_ptr(), b, s, h, hkv, hd, theta, eps,
               _dt(q))
@@ -626,8 +631,7 @@ def qk_norm_rope_backward(q, k, wq, wk, dq_out, dk_out, theta, eps=1e-5, positio
     _same(q, dq_out, dk_out)
     ctx = _on(q, k, wq, wk, positions, dq_out, dk_out)
     ws, n = ctx.workspace("catnn_qk_norm_rope_bwd_workspace", b, s, h, hkv, hd)
-    dq, dk, dw = q.new_empty((b, s, h, hd)), k.new_empty((b, s, hkv, hd)), wq.new_empty((2, hd))
-    dwq, dwk = dw.unbind()
+    dq, dk, dwq, dwk = _dense_like(q), _dense_like(k), torch.empty_like(wq), torch.empty_like(wk)
     _lib.call("catnn_qk_norm_rope_bwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k.data_ptr(), _rows(k, "k"),
               _weight(wq, hd, "wq"), _weight(wk, hd, "wk"), pos, dq_out.data_ptr(), _rows(dq_out, "dq_out"),
               dk_out.data_ptr(), _rows(dk_out, "dk_out"), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
@@ -686,7 +690,7 @@ def kv_append(q, k, v, k_cache, v_cache, page_table, seq_lens, theta, cu_tokens=
     wqp, wkp = (None, None) if wq is None else (_weight(wq, hd, "wq"), _weight(wk, hd, "wk"))
     ctx = _on(k, q, v, k_cache, v_cache, page_table, seq_lens, cu_tokens, wq, wk)
     if q is not None:
-        qo = q.new_empty((t, h, hd))
+        qo = _dense_like(q)
         qop = qo.data_ptr()
     _lib.call("catnn_kv_append", ctx.bind(), qp, q_rows, k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), wqp, wkp,
               qop, k_cache.data_ptr(), v_cache.data_ptr(), table, lens, cu, t, seqs, h, hkv, hd, pages, page, most, theta, eps,

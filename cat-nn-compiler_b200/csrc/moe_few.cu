@@ -145,10 +145,11 @@ struct TcArgs {
     void *h, *y;
     float* yp;        // [runs][T·k, hidden]: each pair's share of y from each run of rows, before its weight
     unsigned* taken;  // [T], then [T·k] weights: what the first kernel found (ALL)
-    unsigned* count;  // [column tiles of hidden]: CTAs that have put theirs there
+    unsigned* count;  // [column tiles of hidden][T]: shares of a token that are there
     int* status;
     int T, hidden, mid, E, k;
     int up_run, down_run;  // rows of a matrix that one CTA takes
+    int counts;
 };
 
 // What routing leaves in shared memory. Pair t·k + i of token t is its i-th
@@ -639,9 +640,8 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     Routes r;
     using S = Tc<T, ALL, 2, NT, BN, CW, ROOM>;
     const S s(a, raw, r, &w1, &w3, a.up_run, a.hidden, a.mid);
-    const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
-    if (first)
-        for (int i = threadIdx.x; i < (a.hidden + 31) / 32; i += S::THREADS) a.count[i] = 0u;
+    if (blockIdx.y == 0 && blockIdx.z == 0)
+        for (int i = blockIdx.x * S::THREADS + threadIdx.x; i < a.counts; i += gridDim.x * S::THREADS) a.count[i] = 0u;
     route_tc<T, NT == 1 ? 1 : 2, CW>(a, s.ring + S::PRE * S::W_BYTES, r, nullptr,
                                   ALL && blockIdx.x < cg::this_cluster().dim_blocks().x && blockIdx.z == 0, [&] { s.prefetch(); });
     find_expert<ALL, CW>(a, blockIdx.z, r);
@@ -678,7 +678,7 @@ template <typename T, bool ALL, int NT, int BN, int CW, int ROOM, int PER_SM>
 __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
     k_down_tc(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap w2) {
     extern __shared__ char raw[];
-    __shared__ bool last;
+    __shared__ bool last[MAX_T];
     Routes r;
     using S = Tc<T, ALL, 1, NT, BN, CW, ROOM>;
     const S s(a, raw, r, &w2, &w2, a.down_run, a.mid, a.hidden);
@@ -708,56 +708,54 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         add_sums<S, 1, NT>((float*)s.ring, t, c, v);
         *(float4*)(a.yp + blockIdx.y * run_size + (i64)r.pair[t] * a.hidden + col0 + c) = v[0];
     }
-    // the last CTA of a column tile adds up what the tokens' experts gave, expert by expert and run by run
+    // Whoever brings the last share of a token's columns adds them up, expert
+    // by expert and run by run, all loads on their way before the first is added.
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.count + blockIdx.x, 1u) == (unsigned)r.active * gridDim.y - 1u;
+    for (int i = threadIdx.x; i < r.n; i += S::THREADS)
+        last[i] = atomicAdd(a.count + blockIdx.x * a.T + r.pair[i] / a.k, 1u) == (unsigned)a.k * gridDim.y - 1u;
     __syncthreads();
-    if (!last) return;
     __threadfence();
-    // A thread's terms (its tokens, their experts, the runs) in one row, eight of them on their way at a time.
     constexpr int Q = BN / 4, TEAMS = S::THREADS / Q, FLIGHT = 8;
     const int c = col0 + threadIdx.x % Q * 4, team = threadIdx.x / Q, runs = gridDim.y;
-    if (c >= a.hidden || team >= TEAMS || team >= a.T) return;
-    int left = ((a.T - 1 - team) / TEAMS + 1) * a.k * runs;
-    int lt = team, lj = 0, lq = 0, t = team, j = 0, q = 0;  // of the next term to load, to add
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), y = v;
-    while (left > 0) {
-        float4 u[FLIGHT];
+    if (c >= a.hidden || team >= TEAMS) return;
+#pragma unroll 1
+    for (int i = team; i < r.n; i += TEAMS) {
+        if (!last[i]) continue;
+        const int t = r.pair[i] / a.k;
+        const float* p = a.yp + (i64)t * a.k * a.hidden + c;
+        int lj = 0, lq = 0, j = 0, q = 0;  // of the next share to load, to add
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), y = v;
+#pragma unroll 1
+        for (int left = a.k * runs; left > 0; left -= FLIGHT) {
+            float4 u[FLIGHT];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            if (i >= left) break;
-            u[i] = __ldcg((const float4*)(a.yp + lq * run_size + ((i64)lt * a.k + lj) * a.hidden + c));
-            if (++lq == runs) {
-                lq = 0;
-                if (++lj == a.k) lj = 0, lt += TEAMS;
+            for (int f = 0; f < FLIGHT; ++f) {
+                if (f >= left) break;
+                u[f] = __ldcg((const float4*)(p + lq * run_size + (i64)lj * a.hidden));
+                if (++lq == runs) lq = 0, ++lj;
             }
-        }
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i) {
-            if (i >= left) break;
-            v.x += u[i].x;
-            v.y += u[i].y;
-            v.z += u[i].z;
-            v.w += u[i].w;
-            if (++q == runs) {
-                const float w = r.w[t * a.k + j];
-                y.x = fmaf(w, v.x, y.x);
-                y.y = fmaf(w, v.y, y.y);
-                y.z = fmaf(w, v.z, y.z);
-                y.w = fmaf(w, v.w, y.w);
-                v = make_float4(0.f, 0.f, 0.f, 0.f);
-                q = 0;
-                if (++j == a.k) {
-                    const float o[4] = {y.x, y.y, y.z, y.w};
-                    stv<T, 4>((T*)a.y + (i64)t * a.hidden + c, o);
-                    y = v;
-                    j = 0;
-                    t += TEAMS;
+            for (int f = 0; f < FLIGHT; ++f) {
+                if (f >= left) break;
+                v.x += u[f].x;
+                v.y += u[f].y;
+                v.z += u[f].z;
+                v.w += u[f].w;
+                if (++q == runs) {
+                    const float w = r.w[t * a.k + j];
+                    y.x = fmaf(w, v.x, y.x);
+                    y.y = fmaf(w, v.y, y.y);
+                    y.z = fmaf(w, v.z, y.z);
+                    y.w = fmaf(w, v.w, y.w);
+                    v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    q = 0;
+                    ++j;
                 }
             }
         }
-        left -= FLIGHT;
+        const float o[4] = {y.x, y.y, y.z, y.w};
+        stv<T, 4>((T*)a.y + (i64)t * a.hidden + c, o);
     }
 }
 
@@ -836,7 +834,7 @@ template <typename T> static bool slot_is_expert(i64 tokens, i64 E, i64 k) {
 }
 
 // f(Shape) for a problem.
-template <typename T, typename F> static void with_shape(Context* c, i64 tokens, i64 mid, i64 E, i64 k, F f) {
+template <typename T, typename F> static void with_shape(Context* c, i64 tokens, i64 hidden, i64 E, i64 k, F f) {
     const bool all = slot_is_expert<T>(tokens, E, k);
     if constexpr (sizeof(T) == 4) {
         if (tokens <= 8) f(Shape<false, 1, 32, 4, 52 * K, 3, 32, 4, 52 * K, 3>());
@@ -844,10 +842,13 @@ template <typename T, typename F> static void with_shape(Context* c, i64 tokens,
         else if (tokens <= 32) f(Shape<true, 4, 32, 8, 104 * K, 2, 32, 8, 104 * K, 2>());
         else f(Shape<true, 8, 32, 8, 120 * K, 1, 32, 8, 120 * K, 1>());
     } else {
-        // thin tiles, where they fit on the SMs at once, need no cluster to cut their rows
-        if (!all && (i64)cdiv(mid, 32) * tokens * k <= (i64)c->sm_count * 4) f(Shape<false, 1, 32, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
-        else if (!all) f(Shape<false, 1, 64, 4, 52 * K, 4, 64, 4, 52 * K, 4>());
+        // the second product's tiles are as wide as the first's where narrow ones would not fit on the SMs at once
+        // (40 tokens, hidden 2048, mid 704, 16 experts: 41.9 against 38.7 us)
+        const bool wide = (i64)cdiv(hidden, 64) * E > (i64)c->sm_count * 2;
+        if (!all) f(Shape<false, 1, 64, 4, 52 * K, 2, 64, 4, 52 * K, 3>());
+        else if (tokens <= 32 && wide) f(Shape<true, 4, 128, 8, 104 * K, 2, 128, 8, 104 * K, 2>());
         else if (tokens <= 32) f(Shape<true, 4, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
+        else if (wide) f(Shape<true, 8, 128, 8, 104 * K, 2, 128, 8, 104 * K, 2>());
         else f(Shape<true, 8, 128, 8, 104 * K, 2, 64, 4, 104 * K, 2>());
     }
 }
@@ -862,12 +863,12 @@ template <typename T> static int slots_of(i64 tokens, i64 E, i64 k) {
 template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k) {
     Layout l{};
     const int slots = slots_of<Ty>(T, E, k);
-    with_shape<Ty>(c, T, mid, E, k, [&](auto shape) {
+    with_shape<Ty>(c, T, hidden, E, k, [&](auto shape) {
         using P = decltype(shape);
         const Plan d = plan(c, slots, (int)T, false, (int)mid, (int)hidden, P::BD, P::PD);
         l.yp = align256((size_t)T * k * mid * sizeof(Ty));
         l.count = l.yp + align256((size_t)d.grid.y * T * k * hidden * 4);
-        l.taken = l.count + align256((size_t)cdiv(hidden, 32) * 4);
+        l.taken = l.count + align256((size_t)cdiv(hidden, P::BD) * T * 4);
         l.bytes = l.taken + align256((size_t)T * (k + 1) * 4);
     });
     return l;
@@ -875,7 +876,7 @@ template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 m
 
 template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, const void* w3, const void* w2) {
     const int slots = slots_of<T>(a.T, a.E, a.k);
-    with_shape<T>(c, a.T, a.mid, a.E, a.k, [&](auto shape) {
+    with_shape<T>(c, a.T, a.hidden, a.E, a.k, [&](auto shape) {
         using P = decltype(shape);
         using U = Tc<T, P::ALL, 2, P::NT, P::BU, P::CU, P::RU>;
         using D = Tc<T, P::ALL, 1, P::NT, P::BD, P::CD, P::RD>;
@@ -887,6 +888,7 @@ template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, c
         const Plan d = plan(c, slots, a.T, false, a.mid, a.hidden, P::BD, P::PD);
         a.up_run = u.run;
         a.down_run = d.run;
+        a.counts = cdiv(a.hidden, P::BD) * a.T;
         launch(c, k_up_tc<T, P::ALL, P::NT, P::BU, P::CU, P::RU, P::PU>, U::THREADS, u.grid, u.cluster, U::smem(a.T, a.k), false, a,
                m1, m3);
         launch(c, k_down_tc<T, P::ALL, P::NT, P::BD, P::CD, P::RD, P::PD>, D::THREADS, d.grid, d.cluster, D::smem(a.T, a.k), true, a,
@@ -913,7 +915,7 @@ static void moe_few_tc(Context* c, const void* x, const void* gate, const void* 
     char* at = (char*)work;
     run_tc<Ty>(c,
                {x, gate, work, y, (float*)(at + l.yp), (unsigned*)(at + l.taken), (unsigned*)(at + l.count), c->status, (int)T,
-                (int)hidden, (int)mid, (int)E, (int)k, 0, 0},
+                (int)hidden, (int)mid, (int)E, (int)k, 0, 0, 0},
                w1, w3, w2);
 }
 

@@ -41,10 +41,14 @@ int* flag(Context* c, int check, int slot) {
     return c->status + slot;
 }
 
+// Positions of a table, with the tile that follows the last one, stay below 2^31.
 void cache_ok(i64 pages, i64 page, i64 max_pages, const char* what) {
-    shape(in32(pages) && page >= 1 && in32(page) && in32(max_pages) && (max_pages == 0 || page <= INT_MAX / max_pages),
+    shape(in32(pages) && page >= 1 && in32(page) && in32(max_pages) && (max_pages == 0 || page <= (INT_MAX - 1024) / max_pages),
           std::string(what) + ": a table must address fewer than 2^31 positions of pages of at least one slot");
 }
+
+// Whether [p, p + n) and [q, q + m) share a byte.
+bool overlap(const void* p, i64 n, const void* q, i64 m) { return (const char*)p < (const char*)q + m && (const char*)q < (const char*)p + n; }
 
 }  // namespace
 
@@ -187,6 +191,8 @@ int catnn_moe_few_fwd(catnn_ctx* h, const void* x, const void* gate, const void*
           "moe_few: need at most 64 tokens and 1 <= k <= E <= 32");
     if (T == 0) return CATNN_OK;
     need(x && gate && w1s && w3s && w2s && y, "moe_few arguments");
+    const i64 rows = T * hidden * (i64)dsize(dtype);
+    CATNN_CHECK(!overlap(x, rows, y, rows), CATNN_ERR_INVALID, "moe_few: y overlaps x, which both kernels read");
     workspace_ok(workspace, workspace_bytes, moe_few_workspace(c, T, hidden, mid, E, k, dtype), "moe_few");
     moe_few(c, x, gate, w1s, w3s, w2s, y, T, hidden, mid, E, k, dtype, workspace);
     ABI_END

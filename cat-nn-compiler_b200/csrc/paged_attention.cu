@@ -578,12 +578,13 @@ __global__ void __launch_bounds__(JOIN, JOIN == 128 ? 10 : 3) k_paged_join(const
         const int head = (int)(out - b * a.h), kvh = head / group, rt = (head - kvh * group) / a.rows;
         const int row = head - kvh * group - rt * a.rows, tiles = tiles_of(a, b);
         if (a.err && tid == 0 && a.lens[b] > (i64)a.max_pages * a.page) atomicExch(a.err, 1);
-        if (tiles == 0) {
+        const int s = tiles_before(a, c, chunk, b) + (kvh * a.row_tiles + rt) * tiles;
+        if (tiles == 0 || s + tiles > c.total) {  // nothing to attend to (or lengths that changed under the kernel)
             for (int i = tid; i < a.hd; i += JOIN) st((T*)a.o + out * a.hd + i, 0.f);
             if (tid == 0) a.lse[out] = -INFINITY;
             continue;
         }
-        const int s = tiles_before(a, c, chunk, b) + (kvh * a.row_tiles + rt) * tiles, w0 = c.worker(s), w1 = c.worker(s + tiles - 1);
+        const int w0 = c.worker(s), w1 = c.worker(s + tiles - 1);
         if (w0 == w1) continue;
         const int parts = w1 - w0 + 1;
         // the first may have come here from another segment; the others start here

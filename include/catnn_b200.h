@@ -351,7 +351,9 @@ int catnn_paged_attention_fwd(catnn_ctx* ctx, const void* q, int64_t q_stride, c
 
 /* catnn_moe_fwd for at most CATNN_MOE_FEW_MAX_TOKENS rows of x: the same
  * block (router ties to the lower index, E <= 32) in two kernels that read
- * each chosen expert's weights once, with no padding of experts to 128 rows. */
+ * each chosen expert's weights once, with no padding of experts to 128 rows.
+ * y must not overlap x. The second kernel starts beside the first (programmatic
+ * dependent launch), which a stream's other work does not notice. */
 #define CATNN_MOE_FEW_MAX_TOKENS 64
 int catnn_moe_few_workspace(catnn_ctx* ctx, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k, int dtype,
                             size_t* bytes);

@@ -89,7 +89,8 @@ def qk_inputs(seed, dtype, b, s, h, hkv, hd, packed, scale=1.0):
 QK = [  # b, s, h, hkv, hd, packed
     (1, 1, 1, 1, 64, False), (2, 37, 4, 2, 64, True), (1, 5, 16, 4, 128, True), (3, 33, 6, 2, 80, False),
     (2, 9, 3, 3, 96, True), (1, 700, 5, 1, 32, False), (1, 3, 2, 1, 256, True), (2, 4, 3, 1, 2, False),
-    (1, 6, 5, 2, 30, True), (1, 2, 2, 2, 254, False), (1, 17, 7, 7, 16, False), (2, 8, 2, 1, 8, True), (5, 1, 4, 4, 48, True)]
+    (1, 6, 5, 2, 30, True), (1, 2, 2, 2, 254, False), (1, 17, 7, 7, 16, False), (2, 8, 2, 1, 8, True), (5, 1, 4, 4, 48, True),
+    (2, 3001, 16, 4, 128, True), (1, 2500, 19, 3, 96, False)]  # warps with many tokens, tokens of several batches of rows
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
@@ -272,6 +273,34 @@ def test_kv_append(lens, new, h, hkv, hd, page, dtype, norm):
     assert torch.equal(k1, kc) and torch.equal(v1, vc)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_kv_append_long_prompts(dtype):
+    """Prompts of thousands of rows, of which a warp walks many, across
+    sequence ends, sequences without new tokens and page ends."""
+    g = gen(44)
+    new = [1999, 0, 3, 1500, 1, 0, 777]
+    lens = [n + m for n, m in zip(new, [0, 40, 13, 2, 500, 0, 31])]
+    h, hkv, hd, page = 16, 4, 128, 24
+    kc, vc, table, ln = make_cache(g, dtype, lens, hkv, hd, page)
+    t = sum(new)
+    qkv = rand(g, t + 5, (h + 2 * hkv) * hd, dtype=dtype)
+    q, k, v = (x.unflatten(-1, (-1, hd)) for x in qkv.split([h * hd, hkv * hd, hkv * hd], -1))
+    w = 1 + rand(g, 2, hd, scale=0.3)
+    cu = torch.tensor([0] + new).cumsum(0).int().cuda()
+    k0, v0 = kc.clone(), vc.clone()
+    qo = ops.kv_append(q, k, v, kc, vc, table, ln, 1e6, cu_tokens=cu, wq=w[0], wk=w[1], eps=EPS, check=True)
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(new)]).cuda()
+    pos = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, new)]).cuda()
+    at = (table[seq, pos // page].long(), slice(None), pos % page)
+    kr, ks = norm_turn(k[:t], w[1], pos, 1e6)
+    qr, qs = norm_turn(q[:t], w[0], pos, 1e6)
+    within(kc[at], kr, own_rounding(kr, dtype) * (1 + 1e-3) + 64 * u * ks, "keys")
+    within(qo[:t], qr, own_rounding(qr, dtype) * (1 + 1e-3) + 64 * u * qs, "queries")
+    assert torch.equal(vc[at], v[:t]) and not qo[t:].any()
+    k0[at], v0[at] = kc[at], vc[at]
+    assert torch.equal(kc, k0) and torch.equal(vc, v0), "every other slot stays as it was"
+
+
 def test_kv_append_one_token_each_and_idle_sequences():
     g = gen(4)
     kc, vc, table, ln = make_cache(g, BF, [7, 0, 33, -2, 16], 2, 64, 16)
@@ -385,6 +414,27 @@ def test_paged_attention_long(dtype, n, h, hkv, hd, page):
     check_attention(q, kc, vc, table, ln, 0, o, lse)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_paged_attention_many_short_sequences(dtype):
+    """More sequences than one warp's scan counts at once, many of them empty."""
+    g = gen(9)
+    b, page, hd = 20_000, 16, 16
+    lens = torch.randint(-3, 45, (b,), generator=g, device="cuda").int()
+    table = torch.randperm(b * 3, generator=g, device="cuda")[:b * 3].int().view(b, 3).contiguous()
+    kc, vc = rand(g, b * 3, 1, page, hd, dtype=dtype), rand(g, b * 3, 1, page, hd, dtype=dtype)
+    q = rand(g, b, 2, hd, dtype=dtype)
+    o, lse = ops.paged_attention(q, kc, vc, table, lens, check=True)
+    k, v = (x[table.long()].view(b, 3 * page, hd).double() for x in (kc, vc))
+    s = q.double() @ k.transpose(1, 2) / math.sqrt(hd)
+    out = torch.arange(3 * page, device="cuda") >= lens[:, None]
+    p = torch.softmax(s.masked_fill(out[:, None], -math.inf), -1).nan_to_num(0.0)
+    ref, mean = (p @ v).reshape(b, -1), (p @ v.abs()).reshape(b, -1)
+    spread = float((q.double().abs() @ k.abs().transpose(1, 2)).amax()) / math.sqrt(hd)
+    within(o, ref, own_rounding(ref, dtype) * (1 + 1e-3)
+           + (2 * (hd + 8) * u * spread + 64 * u + (U if dtype == BF else 0)) * mean, "o")
+    assert bool((lse[lens <= 0] == -math.inf).all()) and torch.isfinite(lse[lens > 0]).all()
+
+
 def test_paged_attention_large_scores():
     """Scores of hundreds that rise and fall along the sequence: the running
     maximum moves, and what came before it all but vanishes."""
@@ -489,6 +539,7 @@ def test_paged_attention_refusals():
         _lib.call("catnn_paged_attention_fwd", h, *a.values())
     for kw, err in (({"q": None}, InvalidArgument), ({"seqs": -1}, ShapeMismatch), ({"hkv": 0}, ShapeMismatch),
                     ({"h": 3}, ShapeMismatch), ({"page": 0}, ShapeMismatch), ({"page": 2 ** 20, "most": 2 ** 12}, ShapeMismatch),
+                    ({"page": 2 ** 31 - 1}, ShapeMismatch),
                     ({"pages": -1}, ShapeMismatch), ({"seqs": 2, "stride": 8}, ShapeMismatch),
                     ({"seqs": 2 ** 31 - 1}, ShapeMismatch)):
         with pytest.raises(err):
@@ -548,7 +599,8 @@ def check_moe(args, k, y):
 MOE = [  # t, hidden, mid, e, k
     (1, 64, 128, 8, 2), (1, 1024, 512, 8, 2), (2, 256, 512, 8, 2), (3, 8, 8, 2, 1), (7, 256, 512, 8, 2), (8, 72, 200, 4, 4),
     (9, 264, 136, 16, 2), (16, 512, 1000, 32, 4), (17, 128, 128, 1, 1), (33, 256, 384, 8, 3), (64, 512, 256, 8, 2),
-    (64, 64, 64, 4, 1), (5, 33, 47, 3, 2), (2, 1, 1, 2, 2), (40, 136, 72, 32, 8), (64, 24, 1032, 2, 2), (6, 2056, 520, 4, 2)]
+    (64, 64, 64, 4, 1), (5, 33, 47, 3, 2), (2, 1, 1, 2, 2), (40, 136, 72, 32, 8), (64, 24, 1032, 2, 2), (6, 2056, 520, 4, 2),
+    (33, 1024, 72, 32, 2), (12, 1280, 136, 20, 3), (8, 1024, 264, 32, 2), (5, 2048, 64, 6, 1), (1, 72, 3000, 30, 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
@@ -617,7 +669,7 @@ def test_moe_few_beside_moe_and_refusals():
     call()
     for kw, err in (({"T": 65}, ShapeMismatch), ({"T": -1}, ShapeMismatch), ({"k": 9}, ShapeMismatch), ({"e": 33}, ShapeMismatch),
                     ({"n": 16}, InvalidArgument), ({"p": ws.data_ptr() + 64}, InvalidArgument), ({"p": None}, InvalidArgument),
-                    ({"x": None}, InvalidArgument), ({"hid": 0}, ShapeMismatch)):
+                    ({"x": None}, InvalidArgument), ({"hid": 0}, ShapeMismatch), ({"x": y.data_ptr()}, InvalidArgument)):
         with pytest.raises(err):
             call(**kw)
 

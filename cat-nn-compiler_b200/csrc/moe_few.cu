@@ -3,8 +3,15 @@
 //   over those k; y = Σ_j w_j·(silu(x·w1)·(x·w3))·w2 of the j-th expert.
 // The grouped GEMMs of the block for many tokens pad every expert to 128
 // rows and take nine launches; here two kernels read the chosen experts'
-// weights once: the first routes and forms h, the second routes again (from
-// x and gate, cheaper than a third launch) and forms y.
+// weights once, the first forming h, the second y. HBM bounds them while they
+// stream; with few tokens the routing before the stream, the hand-over of h
+// and the last sum take as long again.
+//
+// Measured at hidden 1024, mid 3584, 8 experts, top 2: bf16 1 token 18.9 us
+// (44 MB of weights, 2.3 TB/s), 8 tokens 33.5, 64 tokens 46.8 (176 MB, 3.8
+// TB/s); fp32 1 token 33.5 (88 MB), 16 tokens 95, 64 tokens 264 (352 MB, one
+// CTA an SM, each of whose waves routes). 7 tokens, hidden 256, mid 512, fp32:
+// 13.2 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>

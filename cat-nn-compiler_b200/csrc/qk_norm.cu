@@ -7,7 +7,11 @@
 //   forward  y = R(p)·(x·r·w)
 //   adjoint  g = R(p)ᵀ·dy, x̂ = x·r, dw = Σ_rows g·x̂,
 //            dx = r·(g·w − x̂·mean(g·w·x̂))
-// Every kernel reads its rows once and writes them once, so HBM bounds them.
+// Every kernel reads its rows once and writes them once, so HBM bounds them,
+// and next to it the instructions per value. Measured, bf16: 16384 tokens of
+// 16 + 4 heads of 64 forward 17.0 us (4.9 TB/s, 0.75 of the copy rate), adjoint
+// 27.3 us (4.6 TB/s); append of 14087 tokens of 16 + 2 x 4 heads of 128 with
+// the norm 38.8 us (4.2 TB/s); one token 2.1 us, an append of 32 single ones 4.3.
 //
 // A row is held by the smallest power-of-two group of lanes that takes it in
 // 16-byte pieces (8 bf16 or 4 fp32 values a lane; hd 80 and 96 leave lanes
@@ -28,7 +32,8 @@ constexpr int MAX_HD = 256;
 constexpr int WARPS = 8;
 
 // θ^(-2i/hd) / 2π: the pair's turns per position, in f64 because a far
-// position times a rounded f32 frequency is off by whole radians.
+// position times a rounded f32 frequency is off by more than any rounding
+// (up to 0.06 radians at position 10^6).
 struct Freq {
     double turn[MAX_HD / 2];
 };
@@ -48,7 +53,7 @@ static const Freq& freq_of(Context* c, i64 hd, double theta) {
 // (cos, sin) of the angle pos·turn·2π. The turns are reduced to [-1/2, 1/2]
 // in f64, where what is left is exact to 2^-53·|turns|. fp32 rows take
 // sincospi (2 ulp); bf16 rows the hardware sine, whose error of 2^-21 is far
-// below the 2^-9 of the rounding that follows.
+// below the 2^-8 of the rounding that follows.
 template <typename T> __device__ __forceinline__ float2 cos_sin(int pos, double turn) {
     double t = (double)pos * turn;
     t -= rint(t);

@@ -9,9 +9,9 @@
 //
 // Measured at hidden 1024, mid 3584, 8 experts, top 2: bf16 1 token 18.9 us
 // (44 MB of weights, 2.3 TB/s), 8 tokens 33.5, 64 tokens 46.8 (176 MB, 3.8
-// TB/s); fp32 1 token 33.5 (88 MB), 16 tokens 95, 64 tokens 264 (352 MB, one
-// CTA an SM, each of whose waves routes). 7 tokens, hidden 256, mid 512, fp32:
-// 13.2 us.
+// TB/s); fp32 1 token 28.9 (88 MB), 16 tokens 77, 64 tokens 167 (352 MB; the
+// FMAs of 16 tokens an expert, and 448 tiles on 296 places). 7 tokens, hidden
+// 256, mid 512, fp32: 12.6 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -138,9 +138,12 @@ __global__ void __launch_bounds__(THREADS) k_down_any(const __grid_constant__ Ar
 // reads what the first found (ALL = true).
 //
 // fp32 (multiples of 4) runs the same kernels with other hands: the tensor
-// cores would round to TF32, so lanes are columns and packed FMAs multiply,
-// two k at a time; a warp has one of the matrices and its share of a tile's
-// rows. Its logits are TF32 products all the same, of both halves of every
+// cores would round to TF32, so packed FMAs multiply, two k at a time. A lane
+// has four columns (two of w1 and of w3, or four of w2) of up to 8 or 16
+// tokens; the warps split a tile's rows, and more tokens between them. What
+// bounds it beside HBM is the rows of x, 16 bytes that all lanes read at once
+// cost the registers' port as much as 512: with one column to a lane 64 tokens
+// took 264 us in place of 167 (hidden 1024, mid 3584). Its logits are TF32 products all the same, of both halves of every
 // value (a 21-bit product, as exact as the fp32 sums that it goes into).
 constexpr int BK = 64;
 template <typename T> constexpr int XPITCH = BK * (int)sizeof(T) + 16;
@@ -420,19 +423,28 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r,
 constexpr int MAX_STAGES = 8;
 template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct Tc {
     static constexpr int ES = sizeof(T), BN = BN_, BOX = BN < 128 / ES ? BN : 128 / ES, THREADS = (CW + 1) * 32;
-    // groups of warps that have the same columns (fp32: of one matrix) and split a tile's k
-    static constexpr int KG = ES == 4 ? CW / M : CW * 16 / BN;
-    static_assert(ES == 2 || BN == 32, "fp32: a lane to a column");
+    static constexpr int KG = CW * 16 / BN;    // bf16: groups of warps that have the same columns and split a tile's k
+    static constexpr int G = NT < 4 ? 8 : 16;  // fp32: tokens of a warp at most
+    static constexpr int COLS = M * BN / 32;   // fp32: columns of a lane, those of w1 before those of w3
+    static_assert(ES == 2 || (BN % 32 == 0 && NT * 8 <= G * CW && BK / CW % 4 == 0), "fp32: whole lanes and steps of four rows");
     static constexpr int W_BYTES = M * BK * BN * ES, RED_PITCH = BN + 4;  // bytes; floats
-    static constexpr int RED = M * NT * 8 * RED_PITCH;                   // floats of one group's sums
+    static constexpr int RED = (ES == 4 ? CW * M * G : KG * M * NT * 8) * RED_PITCH;  // floats of all sums
     static constexpr int MIN_STAGES = ROOM / (W_BYTES + NT * 8 * XPITCH<T>);
     static constexpr int PRE = ALL ? (MIN_STAGES < 3 ? MIN_STAGES : 3) : 0;  // stages filled before routing
-    static constexpr int SCRATCH = CW * (RT * MAX_E * 4 + (NT == 1 ? 8 : 4) * 512);
+    static constexpr int SCRATCH = CW * (RT * MAX_E * 4 + (ES == 4 ? 0 : (NT == 1 ? 8 : 4) * 512));
     static_assert(ROOM % 1024 == 0 && MIN_STAGES >= 2, "two stages at least");
-    static_assert(KG * RED * 4 <= ROOM && (M == 1 && ALL ? 0 : PRE * W_BYTES + SCRATCH) <= ROOM,
+    static_assert(RED * 4 <= ROOM && (M == 1 && ALL ? 0 : PRE * W_BYTES + SCRATCH) <= ROOM,
                   "the parts, and routing beside the first stages, lie in the ring");
     static_assert(1024 + ROOM + 2 * MAX_STAGES * 8 + MAX_T * (8 + 4 * MAX_E) <= SMEM_MAX, "smem()'s largest");
     static size_t smem(int tokens, int k) { return 1024 + ROOM + 2 * MAX_STAGES * 8 + routes_bytes(tokens, k); }
+
+    // fp32: a tile's tokens are split over 2^teams(n) teams of warps, G or fewer to each
+    static __device__ __forceinline__ int teams(int n) {
+        return ES == 2 || NT * 8 <= G ? 0 : (n > G) + (n > 2 * G) + (n > 4 * G);
+    }
+    // groups of warps with the same columns and tokens, that split a tile's k; rows of a group's sums of one matrix
+    static __device__ __forceinline__ int groups(int n) { return ES == 4 ? CW >> teams(n) : KG; }
+    static __device__ __forceinline__ int red_rows(int n) { return ES == 4 ? G << teams(n) : NT * 8; }
 
     char* ring;
     uint64_t *full, *empty;
@@ -500,7 +512,8 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
     const int stages = min(MAX_STAGES, ROOM / (S::W_BYTES + xbytes));
     char* const xring = s.ring + stages * S::W_BYTES;
     float acc[F32 ? 1 : M][NT][4];  // bf16: the fragments
-    f2 sum[F32 ? NT * 8 : 1];       // fp32: a token's even and odd k
+    constexpr int COLS = F32 ? S::COLS : 1;
+    f2 sum[F32 ? S::G : 1][COLS];   // fp32: a token's even and odd k
 #pragma unroll
     for (int m = 0; m < (F32 ? 1 : M); ++m)
 #pragma unroll
@@ -508,7 +521,12 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
 #pragma unroll
             for (int u = 0; u < 4; ++u) acc[m][j][u] = 0.f;
 #pragma unroll
-    for (int t = 0; t < (F32 ? NT * 8 : 1); ++t) sum[t] = pack2(0.f, 0.f);
+    for (int t = 0; t < (F32 ? S::G : 1); ++t)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) sum[t][c] = pack2(0.f, 0.f);
+    // fp32: this warp's tokens [t0, t0 + G), of which `per` are its own, and its share of a tile's rows
+    const int teams = S::teams(r.n), kg32 = warp >> teams;
+    const int per = (((r.n + (1 << teams) - 1) >> teams) + 3) & ~3, t0 = (warp & (1 << teams) - 1) * per;
     if (warp == CW) {
         auto tokens = [&](int it, int st) {
             constexpr int P = BK / PIECE<T>;  // 16-byte pieces of a row
@@ -536,27 +554,34 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
         }
     } else if constexpr (F32) {
         wait();
-        constexpr int R = BK / S::KG;  // rows of a tile that a warp takes
-        const int m = warp % M, kg = warp / M;
+        const int share = BK / CW << teams, mine = min(per, r.n - t0);
         for (int it = 0, st = 0, ph = 0; it < iters; ++it) {
-            const int kk = min(BK, s.r1 - s.r0 - it * BK);
+            const int kk = min(BK, s.r1 - s.r0 - it * BK), k1 = min(kk, (kg32 + 1) * share);  // kk is a multiple of 4
             tc::mbar_wait(&s.full[st], ph, a.status, 4, 4000000000ll, false);
-            const float* wt = (const float*)(s.ring + st * S::W_BYTES) + m * BK * BN + lane;
-            const char* xt = xring + st * xbytes;
+            const float* wt = (const float*)(s.ring + st * S::W_BYTES) + lane;
+            const char* xt = xring + st * xbytes + t0 * XPITCH<T>;
+#pragma unroll 1
+            for (int k = kg32 * share; k < k1; k += 4) {
+                f2 w[COLS][2];
 #pragma unroll
-            for (int q = 0; q < R; q += 4) {
-                const int k = kg * R + q;
-                if (k >= kk) break;  // kk is a multiple of 4
-                const f2 w01 = pack2(wt[k * BN], wt[(k + 1) * BN]), w23 = pack2(wt[(k + 2) * BN], wt[(k + 3) * BN]);
+                for (int c = 0; c < COLS; ++c) {  // boxes of 32 columns
+                    const float* wc = wt + (c * BK + k) * 32;
+                    w[c][0] = pack2(wc[0], wc[32]);
+                    w[c][1] = pack2(wc[64], wc[96]);
+                }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (j >= nte) break;
+                for (int t = 0; t < S::G; t += 2) {
+                    if (t >= mine) break;
+                    ulonglong2 x[2];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const ulonglong2 x = *(const ulonglong2*)(xt + (j * 8 + u) * XPITCH<T> + k * 4);
-                        sum[j * 8 + u] = fma2(w01, x.x, sum[j * 8 + u]);
-                        sum[j * 8 + u] = fma2(w23, x.y, sum[j * 8 + u]);
-                    }
+                    for (int u = 0; u < 2; ++u) x[u] = *(const ulonglong2*)(xt + (t + u) * XPITCH<T> + k * 4);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int c = 0; c < COLS; ++c) {
+                            sum[t + u][c] = fma2(w[c][0], x[u].x, sum[t + u][c]);
+                            sum[t + u][c] = fma2(w[c][1], x[u].y, sum[t + u][c]);
+                        }
                 }
             }
             __syncwarp();
@@ -606,13 +631,17 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
     __syncthreads();  // every tile of the ring has landed and been read
     if (warp == CW) return;
     if constexpr (F32) {
-        float* red = (float*)s.ring + warp / M * S::RED + warp % M * NT * 8 * S::RED_PITCH + lane;
+        const int rows = S::red_rows(r.n);
 #pragma unroll
-        for (int t = 0; t < NT * 8; ++t)
-            if (t < r.n) red[t * S::RED_PITCH] = sum2(sum[t]);
+        for (int t = 0; t < S::G; ++t)
+            if (t < per && t0 + t < r.n)
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                    ((float*)s.ring)[((kg32 * M + c / (BN / 32)) * rows + t0 + t) * S::RED_PITCH + c % (BN / 32) * 32 + lane] =
+                        sum2(sum[t][c]);
     } else {
         const int wm = warp % (BN / 16), kg = warp / (BN / 16);
-        float* red = (float*)s.ring + kg * S::RED + wm * 16 + (lane >> 2) + (lane & 3) * 2 * S::RED_PITCH;
+        float* red = (float*)s.ring + kg * M * NT * 8 * S::RED_PITCH + wm * 16 + (lane >> 2) + (lane & 3) * 2 * S::RED_PITCH;
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -625,13 +654,14 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
     }
 }
 
-// Adds to v[m] four columns of token t of one CTA's sums.
-template <typename S, int M, int NT> __device__ __forceinline__ void add_sums(const float* red, int t, int c, float4 (&v)[M]) {
-#pragma unroll
-    for (int g = 0; g < S::KG; ++g)
+// Adds to v[m] four columns of token t of one CTA's sums of n tokens.
+template <typename S, int M> __device__ __forceinline__ void add_sums(const float* red, int n, int t, int c, float4 (&v)[M]) {
+    const int groups = S::groups(n), rows = S::red_rows(n);
+#pragma unroll 4
+    for (int g = 0; g < groups; ++g)
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const float4 w = *(const float4*)(red + g * S::RED + (m * NT * 8 + t) * S::RED_PITCH + c);
+            const float4 w = *(const float4*)(red + ((g * M + m) * rows + t) * S::RED_PITCH + c);
             v[m].x += w.x;
             v[m].y += w.y;
             v[m].z += w.z;
@@ -669,7 +699,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         if (s.col0 + c >= a.mid) continue;
         float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         for (int p = 0; p < runs; ++p)
-            add_sums<S, 2, NT>(runs > 1 ? cl.map_shared_rank((float*)s.ring, p * cx + ix) : (float*)s.ring, t, c, v);
+            add_sums<S, 2>(runs > 1 ? cl.map_shared_rank((float*)s.ring, p * cx + ix) : (float*)s.ring, r.n, t, c, v);
         const float* u = (const float*)&v[0];
         const float* g = (const float*)&v[1];
         float h[4];
@@ -712,7 +742,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         const int t = i / (BN / 4), c = (i - t * (BN / 4)) * 4;
         if (col0 + c >= a.hidden) continue;
         float4 v[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
-        add_sums<S, 1, NT>((float*)s.ring, t, c, v);
+        add_sums<S, 1>((float*)s.ring, r.n, t, c, v);
         *(float4*)(a.yp + blockIdx.y * run_size + (i64)r.pair[t] * a.hidden + col0 + c) = v[0];
     }
     // Whoever brings the last share of a token's columns adds them up, expert
@@ -834,20 +864,28 @@ template <bool ALL_, int NT_, int BU_, int CU_, int RU_, int PU_, int BD_, int C
 // before anything is fetched. With few choices most experts' tiles would be
 // fetched in vain. Hidden 1024, mid 3584, 8 experts, top 2: at 4 tokens 31.4 us
 // found first against 29.8, at 16 tokens 41.4 against 36.4; 8 tokens' top 4 of 32
-// (hidden 512, mid 1000) 38.7 against 26.2. fp32, whose CTAs are many, gains
-// nothing from it at 16 tokens (111 us either way).
+// (hidden 512, mid 1000) 38.7 against 26.2. fp32, whose matrices are twice as
+// long: 4 tokens 55.3 us found first against 57.4, 16 tokens 89.4 against 82.9.
 template <typename T> static bool slot_is_expert(i64 tokens, i64 E, i64 k) {
-    return sizeof(T) == 4 ? tokens > 16 : tokens > 8 || tokens * k >= E;
+    return sizeof(T) == 4 ? tokens > 8 : tokens > 8 || tokens * k >= E;
 }
 
 // f(Shape) for a problem.
-template <typename T, typename F> static void with_shape(Context* c, i64 tokens, i64 hidden, i64 E, i64 k, F f) {
+template <typename T, typename F> static void with_shape(Context* c, i64 tokens, i64 hidden, i64 mid, i64 E, i64 k, F f) {
     const bool all = slot_is_expert<T>(tokens, E, k);
     if constexpr (sizeof(T) == 4) {
-        if (tokens <= 8) f(Shape<false, 1, 32, 4, 52 * K, 3, 32, 4, 52 * K, 3>());
-        else if (!all) f(Shape<false, 2, 32, 4, 52 * K, 4, 32, 4, 52 * K, 4>());
-        else if (tokens <= 32) f(Shape<true, 4, 32, 8, 104 * K, 2, 32, 8, 104 * K, 2>());
-        else f(Shape<true, 8, 32, 8, 120 * K, 1, 32, 8, 120 * K, 1>());
+        // short columns: narrow tiles for more CTAs (7 tokens, hidden 256: 12.6 against 12.9 us; 1 token, hidden 1024:
+        // 30.6 against 28.9). Many tokens: eight warps in one CTA an SM where all tiles fit on the SMs at once, else
+        // two CTAs of four (64 tokens, 8 experts: hidden 512, mid 1024 39.1 against 46.2 us; 1024, 3584 189 against 167).
+        const bool small = hidden <= 256, once = (i64)cdiv(mid, 64) * E <= c->sm_count;
+        if (tokens <= 8 && small) f(Shape<false, 1, 32, 4, 52 * K, 3, 64, 4, 52 * K, 3>());
+        else if (tokens <= 8) f(Shape<false, 1, 64, 4, 72 * K, 3, 128, 4, 72 * K, 3>());
+        else if (tokens <= 16 && small) f(Shape<true, 2, 32, 4, 52 * K, 3, 64, 4, 52 * K, 3>());
+        else if (tokens <= 16) f(Shape<true, 2, 64, 8, 104 * K, 2, 128, 8, 104 * K, 2>());
+        else if (tokens <= 32 && once) f(Shape<true, 4, 64, 8, 120 * K, 1, 128, 8, 120 * K, 1>());
+        else if (tokens <= 32) f(Shape<true, 4, 64, 4, 104 * K, 2, 128, 4, 104 * K, 2>());
+        else if (once) f(Shape<true, 8, 64, 8, 120 * K, 1, 128, 8, 120 * K, 1>());
+        else f(Shape<true, 8, 64, 4, 104 * K, 2, 128, 4, 104 * K, 2>());
     } else {
         // the second product's tiles are as wide as the first's where narrow ones would not fit on the SMs at once
         // (40 tokens, hidden 2048, mid 704, 16 experts: 41.9 against 38.7 us)
@@ -870,7 +908,7 @@ template <typename T> static int slots_of(i64 tokens, i64 E, i64 k) {
 template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k) {
     Layout l{};
     const int slots = slots_of<Ty>(T, E, k);
-    with_shape<Ty>(c, T, hidden, E, k, [&](auto shape) {
+    with_shape<Ty>(c, T, hidden, mid, E, k, [&](auto shape) {
         using P = decltype(shape);
         const Plan d = plan(c, slots, (int)T, false, (int)mid, (int)hidden, P::BD, P::PD);
         l.yp = align256((size_t)T * k * mid * sizeof(Ty));
@@ -883,7 +921,7 @@ template <typename Ty> static Layout layout(Context* c, i64 T, i64 hidden, i64 m
 
 template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, const void* w3, const void* w2) {
     const int slots = slots_of<T>(a.T, a.E, a.k);
-    with_shape<T>(c, a.T, a.hidden, a.E, a.k, [&](auto shape) {
+    with_shape<T>(c, a.T, a.hidden, a.mid, a.E, a.k, [&](auto shape) {
         using P = decltype(shape);
         using U = Tc<T, P::ALL, 2, P::NT, P::BU, P::CU, P::RU>;
         using D = Tc<T, P::ALL, 1, P::NT, P::BD, P::CD, P::RD>;

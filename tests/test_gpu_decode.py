@@ -614,6 +614,15 @@ def test_moe_few(t, hid, mid, e, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("t", [4, 9, 13, 16, 17, 29, 33, 37, 52, 64])
+@pytest.mark.parametrize("hid,mid", [(136, 72), (264, 128), (320, 3200)])
+def test_moe_few_every_token_on_every_expert(t, hid, mid, dtype):
+    """The tokens of an expert at every way to split them, in few tiles and in many."""
+    args = moe_inputs(t * 10 + hid, dtype, t, hid, mid, 3)
+    check_moe(args, 3, ops.moe_few(*args, 3))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 def test_moe_few_ties_and_crowds(dtype):
     """Equal logits go to the lower experts; all tokens on one pair of experts."""
     x, gate, w1, w3, w2 = moe_inputs(11, dtype, 64, 128, 128, 8)

@@ -714,7 +714,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, window=None, chec
     ctx = _on(q, k_cache, v_cache, page_table, seq_lens)
     dt = _dt(q)
     ws, n = ctx.workspace("catnn_paged_attention_workspace", b, h, hkv, hd, dt)
-    o, lse = q.new_empty((b, h * hd)), q.new_empty((b, h), dtype=torch.float32)
+    o, lse = q.new_empty(b, h * hd), torch.empty(b, h, dtype=torch.float32, device=q.device)
     _lib.call("catnn_paged_attention_fwd", ctx.bind(), q.data_ptr(), _rows(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(),
               table, lens, o.data_ptr(), lse.data_ptr(), b, h, hkv, hd, pages, page, most, window or 0, dt,
               ws.data_ptr() if n else None, n, check)

@@ -10,8 +10,8 @@
 // Every kernel reads its rows once and writes them once, so HBM bounds them,
 // and next to it the instructions per value. Measured, bf16: 16384 tokens of
 // 16 + 4 heads of 64 forward 17.0 us (4.9 TB/s, 0.75 of the copy rate), adjoint
-// 27.3 us (4.6 TB/s); append of 14087 tokens of 16 + 2 x 4 heads of 128 with
-// the norm 38.8 us (4.2 TB/s); one token 2.1 us, an append of 32 single ones 4.3.
+// 27.4 us (4.6 TB/s); append of 14087 tokens of 16 + 2 x 4 heads of 128 with
+// the norm 39.9 us (4.1 TB/s); one token 2.7 us, an append of 32 single ones 4.4.
 //
 // A row is held by the smallest power-of-two group of lanes that takes it in
 // 16-byte pieces (8 bf16 or 4 fp32 values a lane; hd 80 and 96 leave lanes

@@ -615,7 +615,7 @@ def test_moe_few(t, hid, mid, e, k, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("t", [4, 9, 13, 16, 17, 29, 33, 37, 52, 64])
-@pytest.mark.parametrize("hid,mid", [(136, 72), (264, 128), (320, 3200)])
+@pytest.mark.parametrize("hid,mid", [(136, 72), (264, 128), (320, 3200), (2056, 72)])
 def test_moe_few_every_token_on_every_expert(t, hid, mid, dtype):
     """The tokens of an expert at every way to split them, in few tiles and in many."""
     args = moe_inputs(t * 10 + hid, dtype, t, hid, mid, 3)

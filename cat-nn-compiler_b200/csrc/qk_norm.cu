@@ -23,13 +23,15 @@
 
 #include "ops.cuh"
 #include "paged_place.cuh"
+#include "row_deal.cuh"
 #include "tc_prims.cuh"
 
 namespace catnn {
 namespace qkn {
 
+using namespace deal;
+
 constexpr int MAX_HD = 256;
-constexpr int WARPS = 8;
 
 // θ^(-2i/hd) / 2π: the pair's turns per position, in f64 because a far
 // position times a rounded f32 frequency is off by more than any rounding
@@ -179,34 +181,8 @@ __device__ __forceinline__ void load_weights(float (&sw)[2][MAX_HD], const float
     __syncthreads();
 }
 
-// How the row groups of all tokens are dealt out to the warps of a grid: a
-// token's groups to `parts` warps, `per` to each. Such a team takes every
-// teams-th token (run = 0: all warps then read along one front, 17.1 us where
-// runs took 18.1 for 16384 tokens of 16 + 4 heads of 64), or a run of
-// neighbours, where one look-up serves many (the append: 39 against 43 us).
-struct Deal {
-    int tokens, groups, parts, per, run, teams;
-};
-struct Share {
-    int t0, t1, dt, g0, g1;
-};
-__device__ __forceinline__ Share share_of(const Deal& d) {
-    const int w = blockIdx.x * WARPS + (threadIdx.x >> 5), team = w / d.parts, part = w - team * d.parts;
-    Share s;
-    if (team >= d.teams) {
-        s.t0 = s.t1 = 0;
-    } else if (d.run == 0) {
-        s.t0 = team;
-        s.t1 = d.tokens;
-    } else {
-        s.t0 = (int)min((i64)d.tokens, (i64)team * d.run);
-        s.t1 = (int)min((i64)d.tokens, (i64)s.t0 + d.run);
-    }
-    s.dt = d.run == 0 ? d.teams : 1;
-    s.g0 = part * d.per;
-    s.g1 = min(d.groups, s.g0 + d.per);
-    return s;
-}
+// A warp's share of the rows (row_deal.cuh).
+__device__ __forceinline__ Share my_share(const Deal& d) { return share_of(d, blockIdx.x * WARPS + (threadIdx.x >> 5)); }
 
 struct FwdArgs {
     const void *q, *k;
@@ -232,7 +208,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) k_qk_fwd(const __grid_constant_
     const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd;
     load_weights(sw, a.wq, a.wk, a.hd);
-    const Share w = share_of(a.deal);
+    const Share w = my_share(a.deal);
     for (int tok = w.t0; tok < w.t1; tok += w.dt) {
         Turn<T> t;
         for (int g0 = w.g0; g0 < w.g1; g0 += BATCH) {
@@ -334,7 +310,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) k_qk_bwd(const __grid_constant_
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[m][0][j] = acc[m][1][j] = pack2(0.f, 0.f);
     const f2 minus = pack2(-1.f, -1.f);
-    const Share w = share_of(a.deal);
+    const Share w = my_share(a.deal);
     for (int tok = w.t0; tok < w.t1; tok += w.dt) {
       Turn<T> t;
       f2 ns[N];
@@ -555,7 +531,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) k_append(const __grid_constant_
     const int lane = threadIdx.x & 31, sub = lane / LPH, e0 = lane % LPH * V, step = HPW * a.hd, off = sub * a.hd + e0;
     const bool in = e0 < a.hd, norm = a.wq != nullptr;
     load_weights(sw, a.wq, a.wk, a.hd);
-    const Share w = share_of(a.deal);
+    const Share w = my_share(a.deal);
     place::Token at;
     for (int tok = w.t0; tok < w.t1; tok += w.dt) {
         Turn<T> t;
@@ -650,21 +626,6 @@ __global__ void __launch_bounds__(WARPS * 32) k_append_any(const __grid_constant
 }
 
 // ------------------------------------------------------------ launchers
-// A warp takes all groups of its tokens (whose sines and places are then found
-// once a token) unless that would leave SMs without warps. -> the grid, up to
-// `per_sm` CTAs an SM.
-static int deal_out(Context* c, i64 tokens, int groups, int per_sm, bool runs, Deal& d) {
-    const i64 want = (i64)c->sm_count * 16, most = (i64)c->sm_count * per_sm;
-    d.tokens = (int)tokens;
-    d.groups = groups;
-    d.per = (int)std::max<i64>(1, std::min<i64>(groups, tokens * groups / want));
-    d.parts = cdiv(groups, d.per);
-    const i64 ctas = std::min(most, (tokens * d.parts + WARPS - 1) / WARPS);
-    d.teams = (int)std::max<i64>(1, std::min(tokens, ctas * WARPS / d.parts));
-    d.run = runs ? cdiv(tokens, d.teams) : 0;
-    return (int)(((i64)d.teams * d.parts + WARPS - 1) / WARPS);
-}
-
 static int lanes_of(int hd, int vec) {
     int l = 4;
     while (l * vec < hd) l <<= 1;
@@ -712,7 +673,7 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && aligned_to(qo, 16) &&
         aligned_to(ko, 16)) {
         a.gq = cdiv(h, 32 / lph);
-        const int grid = deal_out(c, tokens, a.gq + cdiv(hkv, 32 / lph), 3, false, a.deal);
+        const int grid = deal_out(c->sm_count, tokens, a.gq + cdiv(hkv, 32 / lph), 3, false, a.deal);
 #define RUN(T, L) k_qk_fwd<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
@@ -724,11 +685,8 @@ void qk_norm_rope_fwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     launched(c);
 }
 
-// CTAs of the adjoint: what the SMs hold at once, each walking many tokens,
-// because every CTA adds a row to each weight sum.
-constexpr int BWD_PER_SM = 2;
 size_t qk_norm_rope_bwd_workspace(Context* c, i64 b, i64 s, i64 h, i64 hkv, i64 hd) {
-    return (size_t)std::min<i64>((i64)c->sm_count * BWD_PER_SM, b * s * (h + hkv)) * 2 * hd * sizeof(float);
+    return (size_t)adjoint_rows(c->sm_count, b * s, h + hkv) * 2 * hd * sizeof(float);
 }
 
 void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i64 k_stride, const float* wq, const float* wk,
@@ -741,17 +699,21 @@ void qk_norm_rope_bwd(Context* c, const void* q, i64 q_stride, const void* k, i6
     BwdArgs a{q, k, gq, gk, q_stride, k_stride, gq_stride, gk_stride, wq, wk, pos, dq, dk, work, tokens, s, (int)h, (int)hkv,
               (int)hd, eps, 1.f / (float)hd, {}, 0};
     int ctas = 0;
+    const i64 room = adjoint_rows(c->sm_count, tokens, h + hkv);  // rows of each weight sum in `work`
+    const auto fits = [&] { CATNN_CHECK(ctas <= room, CATNN_ERR_INVALID, "qk_norm_rope backward: more CTAs than the workspace has rows"); };
     if (tokens > 0) {
         const int vec = dtype == CATNN_BF16 ? 8 : 4, lph = lanes_of((int)hd, vec);
         if (lph <= 32 && rows_ok(q, q_stride, hd, vec) && rows_ok(k, k_stride, hd, vec) && rows_ok(gq, gq_stride, hd, vec) &&
             rows_ok(gk, gk_stride, hd, vec) && aligned_to(dq, 16) && aligned_to(dk, 16)) {
             a.groups_q = cdiv(h, 32 / lph);
-            ctas = deal_out(c, tokens, a.groups_q + cdiv(hkv, 32 / lph), BWD_PER_SM, false, a.deal);
+            ctas = deal_out(c->sm_count, tokens, a.groups_q + cdiv(hkv, 32 / lph), ADJOINT_PER_SM, false, a.deal);
+            fits();
 #define RUN(T, L) k_qk_bwd<T, L><<<ctas, WARPS * 32, 0, c->stream>>>(a, f)
             if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN
         } else {
-            ctas = (int)std::min<i64>((i64)c->sm_count * BWD_PER_SM, (tokens * (h + hkv) + WARPS - 1) / WARPS);
+            ctas = (int)std::min<i64>((i64)c->sm_count * ADJOINT_PER_SM, (tokens * (h + hkv) + WARPS - 1) / WARPS);
+            fits();
             if (dtype == CATNN_BF16) k_qk_bwd_any<bf16><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
             else k_qk_bwd_any<float><<<ctas, WARPS * 32, 0, c->stream>>>(a, f);
         }
@@ -784,7 +746,7 @@ void kv_append(Context* c, const void* q, i64 q_stride, const void* k, i64 k_str
         aligned_to(qo, 16) && aligned_to(kc, 16) && aligned_to(vc, 16)) {
         a.gq = cdiv(h, 32 / lph);
         a.gk = cdiv(hkv, 32 / lph);
-        const int grid = deal_out(c, tokens, a.gq + 2 * a.gk, 3, true, a.deal);
+        const int grid = deal_out(c->sm_count, tokens, a.gq + 2 * a.gk, 3, true, a.deal);
 #define RUN(T, L) k_append<T, L><<<grid, WARPS * 32, 0, c->stream>>>(a, f)
         if (dtype == CATNN_BF16) { BY_LANES(lph, RUN, bf16) } else { BY_LANES(lph, RUN, float) }
 #undef RUN

@@ -685,9 +685,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_paged_any(const __grid_constant_
             if (d < a.hd) s = fmaf(q[u], ld((const T*)a.kc + row + d), s);
         }
         s = warp_sum(s);
-        const float mn = fmaxf(m, s);
-        if (mn == -INFINITY) continue;
-        const float keep = expf(m - mn), p = expf(s - mn);
+        // a NaN score leaves the maximum and makes its weight NaN; while all are -inf their weights are 0
+        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
+        const float keep = expf(m - base), p = expf(s - base);
         l = l * keep + p;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -706,12 +706,13 @@ __global__ void __launch_bounds__(WARPS * 32) k_paged_any(const __grid_constant_
     float top = -INFINITY, total = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm[w]);
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += sl[w] != 0.f ? sl[w] * expf(sm[w] - top) : 0.f;
+    for (int w = 0; w < WARPS; ++w) total = fmaf(sl[w], expf(sm[w] - base), total);
     for (int d = threadIdx.x; d < a.hd; d += WARPS * 32) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) v += sl[w] != 0.f ? so[w][d] * expf(sm[w] - top) : 0.f;
+        for (int w = 0; w < WARPS; ++w) v = fmaf(so[w][d], expf(sm[w] - base), v);
         st((T*)a.o + (b * a.h + head) * a.hd + d, total != 0.f ? v / total : 0.f);
     }
     if (threadIdx.x == 0) a.lse[b * a.h + head] = total != 0.f ? top + logf(total) : -INFINITY;

@@ -8,7 +8,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import BF, D, EPS, F32, U, inv_rms, own_rounding, pair_size, qk_inputs, rand, gen, turn, u, within
+from test_gpu_decode import (BF, EPS, F32, U, gather, gen, inv_rms, make_cache,
+                             own_rounding, pair_size, qk_inputs, rand, turn, u, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,84 @@ def test_qk_norm_rope_backward_of_a_token_with_more_heads_than_the_grid_has_warp
         scale = r * (size * w.abs() + xh.abs() * (size * w.abs() * xh.abs()).mean(-1, keepdim=True))
         within(dx, ref, own_rounding(ref, dtype) * (1 + 1e-3) + 64 * u * scale, f"d{what}")
         within(dw, (t * xh).flatten(0, 2).sum(0), 192 * u * (size * xh.abs()).flatten(0, 2).sum(0), f"dw{what}")
+
+
+# ------------------------------------------------------------------ infinities and NaN, on every path
+#: dtype, head size, whether the caches start off a 16-byte boundary: tensor cores, FMA, and any size and alignment
+PATHS = [(BF, 64, False), (F32, 64, False), (BF, 7, False), (F32, 7, False), (BF, 64, True), (F32, 64, True)]
+
+
+def off_boundary(t):
+    """t's values in memory that starts one element off a 16-byte boundary."""
+    room = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    out = room[1:].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+def plain_attention(q, kc, vc, table, n):
+    """softmax(q·Kᵀ/√hd)·V of sequence 0 in 64 bits, with what infinities and NaN make of it."""
+    h, hd, hkv = q.shape[1], q.shape[2], kc.shape[1]
+    k, v = gather(kc, table, 0, 0, n).double(), gather(vc, table, 0, 0, n).double()
+    s = torch.einsum("ngd,jnd->ngj", q[0].double().view(hkv, h // hkv, hd), k) / math.sqrt(hd)
+    return torch.einsum("ngj,jnd->ngd", torch.softmax(s, -1), v).reshape(-1), torch.logsumexp(s, -1).reshape(-1)
+
+
+@pytest.mark.parametrize("dtype,hd,off", PATHS)
+@pytest.mark.parametrize("what", ["query", "first key", "early key", "late key", "every key", "value", "value of no weight",
+                                  "infinite score"])
+def test_paged_attention_shows_nan_on_every_path(what, dtype, hd, off):
+    """A NaN shows in the heads that meet it, in every kernel, wherever it stands, and in no others."""
+    g = gen(71)
+    kc, vc, table, ln = make_cache(g, dtype, [300, 40], 2, hd, 16)
+    q = rand(g, 2, 4, hd, dtype=dtype).abs() + 0.25
+
+    def put(cache, j, value):  # into kv head 0 of sequence 0
+        cache[table[0, j // 16], 0, j % 16] = value
+    if what == "query":
+        q[0, 0, hd - 1] = math.nan
+    elif what == "every key":
+        for j in range(300):
+            put(kc, j, math.nan)
+    elif what == "value":
+        put(vc, 123, math.nan)
+    elif what == "value of no weight":
+        put(kc, 123, -math.inf)
+        put(vc, 123, math.inf)
+    elif what == "infinite score":
+        put(kc, 5, math.inf)
+    else:
+        put(kc, {"first key": 0, "early key": 9, "late key": 299}[what], math.nan)
+    if off:
+        kc, vc = off_boundary(kc), off_boundary(vc)
+    o, lse = ops.paged_attention(q, kc, vc, table, ln)
+    ref, rl = plain_attention(q, kc, vc, table, 300)
+    assert torch.equal(torch.isnan(o[0]), torch.isnan(ref)) and torch.isnan(ref).any() and not torch.isnan(ref).all()
+    if what != "infinite score":  # there the largest score alone is known to be infinite
+        assert torch.equal(torch.isnan(lse[0]), torch.isnan(rl))
+    assert torch.isfinite(o[1]).all() and torch.isfinite(lse[1]).all()
+
+
+@pytest.mark.parametrize("dtype,hd,off", PATHS)
+def test_paged_attention_infinite_scores_on_every_path(dtype, hd, off):
+    """Scores of -inf take no weight, wherever they stand; a sequence of nothing else gets zeros and -inf."""
+    g = gen(72)
+    kc, vc, table, ln = make_cache(g, dtype, [100, 40], 1, hd, 16)
+    q = rand(g, 2, 2, hd, dtype=dtype).abs() + 0.5
+    gone = [0, 1, 8, 40, 99]
+    for b, js in ((0, gone), (1, range(40))):
+        for j in js:
+            kc[table[b, j // 16], :, j % 16] = -math.inf
+    if off:
+        kc, vc = off_boundary(kc), off_boundary(vc)
+    o, lse = ops.paged_attention(q, kc, vc, table, ln)
+    assert not o[1].any() and bool((lse[1] == -math.inf).all())
+    keep = torch.tensor([j for j in range(100) if j not in gone], device="cuda")
+    k, v = gather(kc, table, 0, 0, 100)[keep, 0].double(), gather(vc, table, 0, 0, 100)[keep, 0].double()
+    s = q[0].double() @ k.T / math.sqrt(hd)
+    p = torch.softmax(s, -1)
+    # the counts of check_attention: a score's roundings twice, 66 of the sums, P in bf16
+    spread = float((q[0].double().abs() @ k.abs().T).amax()) / math.sqrt(hd)
+    mean = p @ v.abs()
+    within(o[0].view(2, hd), p @ v, own_rounding(p @ v, dtype) * (1 + 1e-3)
+           + (2 * (hd + 8) * u * spread + 66 * u + (U if dtype == BF else 0)) * mean, "o")

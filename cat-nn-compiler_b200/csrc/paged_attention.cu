@@ -49,11 +49,12 @@ struct Args {
     float *part, *ml;                     // [workers][2][rows][pitch] sums, [workers][2][rows][2] maximum and weight
 };
 
-// The positions [first, len) that sequence b attends to.
+// The positions [first, len) that sequence b attends to: its window, as far as
+// the table holds it (nothing, where the window lies beyond the table).
 __device__ __forceinline__ void span_of(const Args& a, i64 b, int& first, int& len) {
-    const i64 held = (i64)a.max_pages * a.page;
-    len = (int)min(held, (i64)max(a.lens[b], 0));
-    first = a.window > 0 && len > a.window ? len - a.window : 0;
+    const int held = a.max_pages * a.page, all = max(a.lens[b], 0);  // a table's positions stay below 2^31
+    len = min(held, all);
+    first = a.window > 0 && all > a.window ? min(all - a.window, len) : 0;
 }
 __device__ __forceinline__ int tiles_of(const Args& a, i64 b) {  // of one segment
     int first, len;

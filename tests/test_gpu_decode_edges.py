@@ -8,12 +8,13 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import (BF, EPS, F32, U, gather, gen, inv_rms, make_cache,
+from test_gpu_decode import (BF, EPS, F32, U, check_attention, gather, gen, inv_rms, make_cache,
                              own_rounding, pair_size, qk_inputs, rand, turn, u, within)
 
 pytestmark = pytest.mark.gpu
 
 from catnn_b200 import _lib, ops  # noqa: E402
+from catnn_b200.errors import ShapeMismatch  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -129,3 +130,25 @@ def test_paged_attention_infinite_scores_on_every_path(dtype, hd, off):
     mean = p @ v.abs()
     within(o[0].view(2, hd), p @ v, own_rounding(p @ v, dtype) * (1 + 1e-3)
            + (2 * (hd + 8) * u * spread + 66 * u + (U if dtype == BF else 0)) * mean, "o")
+
+
+@pytest.mark.parametrize("dtype,hd,off", PATHS)
+def test_paged_attention_windows_beyond_the_table(dtype, hd, off):
+    """A sequence longer than its table: the positions of its window that the
+    table does not hold are left out, and none before the window comes in for them."""
+    g = gen(73)
+    kc, vc, table, _ = make_cache(g, dtype, [64, 64, 64, 64], 2, hd, 16)
+    q = rand(g, 4, 4, hd, dtype=dtype)
+    if off:
+        kc, vc = off_boundary(kc), off_boundary(vc)
+    ln = torch.tensor([1000, 70, 64, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    o, lse = ops.paged_attention(q, kc, vc, table, ln, window=16)
+    assert not o[0].any() and not o[3].any() and bool((lse[[0, 3]] == -math.inf).all())
+    # positions 54 to 63 of sequence 1: what a length of 64 attends to with a window of 10
+    held = torch.full_like(ln, 64)
+    short, sl = ops.paged_attention(q, kc, vc, table, held, window=10)
+    check_attention(q[1:2], kc, vc, table[1:2], held[1:2], 10, o[1:2], lse[1:2])
+    check_attention(q[1:2], kc, vc, table[1:2], held[1:2], 10, short[1:2], sl[1:2])
+    check_attention(q[2:3], kc, vc, table[2:3], held[2:3], 16, o[2:3], lse[2:3])
+    with pytest.raises(ShapeMismatch, match="no page"):
+        ops.paged_attention(q, kc, vc, table, ln, window=16, check=True)

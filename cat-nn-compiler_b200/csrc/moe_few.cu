@@ -213,6 +213,25 @@ __device__ __forceinline__ unsigned choose(float l, int E, int k, int lane, floa
     return taken;
 }
 
+// fp32 logits of token t by a warp, lane e holding expert e's: an infinite
+// value, or one that TF32 rounds to infinity, leaves NaN as its lower half,
+// so logits that came out NaN are added up again from the values as they are
+// (an expert shut off by -inf then has the logit -inf; a NaN of the inputs'
+// stays one).
+__device__ __forceinline__ float exact_where_nan(const TcArgs& a, int t, float l) {
+    const int lane = threadIdx.x & 31;
+    for (unsigned left = __ballot_sync(0xffffffffu, l != l); left; left &= left - 1) {
+        const int e = __ffs(left) - 1;
+        float s = 0.f;
+#pragma unroll 4
+        for (int i = lane; i < a.hidden; i += 32)
+            s = fmaf(((const float*)a.x)[(i64)t * a.hidden + i], ((const float*)a.gate)[(i64)i * a.E + e], s);
+        s = warp_sum(s);
+        if (lane == e) l = s;
+    }
+    return l;
+}
+
 // `issued` is called by every warp when its first batch's loads are on their way.
 template <int R8, int CW, typename Issued>
 __device__ __forceinline__ void logits_f32(const TcArgs& a, int t0, int rows, float* part, Issued issued) {
@@ -396,8 +415,9 @@ __device__ __forceinline__ void route_tc(const TcArgs& a, char* room, Routes& r,
         if (lane < a.E)
 #pragma unroll
             for (int w = 0; w < CW; ++w) l += part[(w * RT + i) * ep + lane];
-        const unsigned taken = choose(l, a.E, a.k, lane, top);
         const int t = t0 + i;
+        if constexpr (sizeof(T) == 4) l = exact_where_nan(a, t, l);
+        const unsigned taken = choose(l, a.E, a.k, lane, top);
         if (lane < copies) to[t] = taken;
         if (w_here || tell) {
             const bool in = taken >> lane & 1u;

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import (BF, EPS, F32, U, check_attention, gather, gen, inv_rms, make_cache,
+from test_gpu_decode import (BF, EPS, F32, U, check_attention, check_moe, gather, gen, inv_rms, make_cache, moe_inputs,
                              own_rounding, pair_size, qk_inputs, rand, turn, u, within)
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +152,28 @@ def test_paged_attention_windows_beyond_the_table(dtype, hd, off):
     check_attention(q[2:3], kc, vc, table[2:3], held[2:3], 16, o[2:3], lse[2:3])
     with pytest.raises(ShapeMismatch, match="no page"):
         ops.paged_attention(q, kc, vc, table, ln, window=16, check=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("t,hid,mid,e", [(1, 128, 128, 8), (7, 128, 136, 8), (12, 136, 128, 6), (40, 256, 128, 32), (5, 24, 40, 8),
+                                         (3, 130, 66, 5)])
+def test_moe_few_experts_shut_off(t, hid, mid, e, dtype):
+    """Experts whose logit is -inf, or the type's lowest value, are taken by
+    nobody; an infinite row of x leaves the other rows as they are."""
+    x, gate, w1, w3, w2 = moe_inputs(74 + hid, dtype, t, hid, mid, e)
+    x[:, 0] = 1.0
+    for low in (-math.inf, torch.finfo(dtype).min):
+        for shut in ([0], [e - 1], [0, 2, 3]):
+            off = gate.clone()
+            off[0, shut] = low
+            y = ops.moe_few(x, off, w1, w3, w2, 2)
+            clean = gate.clone()
+            clean[0, shut] = -1e4  # far below every other logit
+            check_moe((x, clean, w1, w3, w2), 2, y)
+    if t > 1:
+        y = ops.moe_few(x, gate, w1, w3, w2, 2)
+        bad = x.clone()
+        bad[1, 5] = math.inf
+        y2 = ops.moe_few(bad, gate, w1, w3, w2, 2)
+        others = [i for i in range(t) if i != 1]
+        assert torch.equal(y2[others], y[others]) and not torch.isfinite(y2[1]).all()

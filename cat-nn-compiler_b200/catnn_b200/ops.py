@@ -26,14 +26,12 @@ class Context:
         h = C.c_void_p()
         _lib.call("catnn_ctx_create", int(device), C.byref(h))
         self.handle = h
-        self._stream = None
         self._workspace = {}
 
     def bind(self):
-        s = torch._C._cuda_getCurrentRawStream(self.device)
-        if s != self._stream:
-            _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
-            self._stream = s
+        # set on every call: another thread, or a caller of the C ABI, may have set another one since
+        s = torch.cuda.current_stream(self.device).cuda_stream
+        _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
         return self.handle
 
     def workspace(self, name, *sizes):

@@ -73,3 +73,33 @@ def test_a_grid_has_every_row_once(deal):
                int(r.integers(0, 2))) for _ in range(200)]
     for c in cases:
         assert deal.covers(*c), c
+
+
+def test_bind_sets_the_stream_every_time(monkeypatch):
+    """The handle's stream is what the caller's is, whoever set it last: another
+    thread between two calls, or a caller through the C ABI."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from catnn_b200 import _lib, ops
+    handle = {"stream": None}
+    now = {"stream": 0}
+
+    def call(name, *args):
+        if name == "catnn_ctx_set_stream":
+            handle["stream"] = args[1].value or 0
+        elif name == "catnn_ctx_create":
+            args[1]._obj.value = 1234
+        return 0
+    monkeypatch.setattr(_lib, "call", call)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=now["stream"]))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: now["stream"], raising=False)
+    ctx = ops.Context(0)
+    for mine, other in ((0, 64), (64, 0), (64, 128), (128, 128)):
+        now["stream"] = mine
+        ctx.bind()
+        assert handle["stream"] == mine
+        handle["stream"] = other  # behind the context's back
+        ctx.bind()
+        assert handle["stream"] == mine

@@ -52,8 +52,9 @@ struct Args {
 // The positions [first, len) that sequence b attends to: its window, as far as
 // the table holds it (nothing, where the window lies beyond the table).
 __device__ __forceinline__ void span_of(const Args& a, i64 b, int& first, int& len) {
-    const int held = a.max_pages * a.page, all = max(a.lens[b], 0);  // a table's positions stay below 2^31
-    len = min(held, all);
+    const i64 held = (i64)a.max_pages * a.page;  // (with 32 bits k_paged_fma is compiled to 25.3 us in place of 21.3 on the long case)
+    const int all = max(a.lens[b], 0);
+    len = (int)min(held, (i64)all);
     first = a.window > 0 && all > a.window ? min(all - a.window, len) : 0;
 }
 __device__ __forceinline__ int tiles_of(const Args& a, i64 b) {  // of one segment

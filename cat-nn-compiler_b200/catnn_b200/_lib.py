@@ -80,6 +80,8 @@ SIGNATURES = {
                                   C.c_size_t, I32],
     "catnn_moe_few_workspace": [VP, I64, I64, I64, I64, I64, I32, C.POINTER(C.c_size_t)],
     "catnn_moe_few_fwd": [VP, VP, VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I32, VP, C.c_size_t],
+    "catnn_moe_few_set_timeout_ms": [VP, I64],
+    "catnn_moe_few_check": [VP],
     "catnn_sgd": [VP, VP, VP, I64, F32, VP],
     "catnn_adam": [VP, VP, VP, VP, VP, I64, U64, F32, F32, F32, F32, I32, VP],
     "catnn_mlp_step": [VP, VP, VP, VP, VP, VP, VP, VP, I32, I64, I64, I64, I64, VP, VP, VP, VP, VP],

@@ -719,9 +719,11 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, window=None, chec
     return o, lse
 
 
-def moe_few(x, gate, w1s, w3s, w2s, top_k):
+def moe_few(x, gate, w1s, w3s, w2s, top_k, check=False):
     """moe() for at most 64 rows of x, in two kernels that read each chosen
-    expert's weights once; expert weights stacked [E, ...]."""
+    expert's weights once; expert weights stacked [E, ...]. check=True
+    (synchronizing) reports a bounded wait that ran out, in this call or one
+    since the last check, as a DeviceTimeout; its rows are NaN."""
     _same(x, gate, w1s, w3s, w2s)
     ws1 = w1s.shape
     hid = x.shape[-1]
@@ -743,6 +745,8 @@ def moe_few(x, gate, w1s, w3s, w2s, top_k):
     y = torch.empty_like(x)
     _lib.call("catnn_moe_few_fwd", ctx.bind(), x.data_ptr(), gate.data_ptr(), w1s.data_ptr(), w3s.data_ptr(),
               w2s.data_ptr(), y.data_ptr(), t, hid, mid, e, top_k, dt, ws.data_ptr() if n else None, n)
+    if check:
+        _lib.call("catnn_moe_few_check", ctx.handle)
     return y
 
 

@@ -198,4 +198,18 @@ int catnn_moe_few_fwd(catnn_ctx* h, const void* x, const void* gate, const void*
     ABI_END
 }
 
+int catnn_moe_few_set_timeout_ms(catnn_ctx* h, int64_t ms) {
+    ABI_BEGIN
+    Context* c = unwrap(h);
+    CATNN_CHECK(ms >= 0 && ms <= 3600000, CATNN_ERR_INVALID, "moe_few: timeout must be in [0, 3600000] ms");
+    c->few_patience = ms * 2000000ll;  // cycles at 2 GHz
+    ABI_END
+}
+
+int catnn_moe_few_check(catnn_ctx* h) {
+    ABI_BEGIN
+    if (take_status(unwrap(h), FEW_STATUS_SLOT)) throw Error(CATNN_ERR_TIMEOUT, "moe_few: a bounded device wait ran out");
+    ABI_END
+}
+
 }  // extern "C"

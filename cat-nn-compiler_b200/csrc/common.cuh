@@ -60,6 +60,8 @@ struct Context {
     double turns[128] = {0.0};
     i64 turns_hd = 0;
     double turns_theta = 0.0;
+    // Cycles after which a wait of the MoE for a few tokens gives up (moe_few.cu); about 2 s.
+    long long few_patience = 4000000000ll;
     // Grow-only arena for composite ops (several temporaries held across
     // the leaf launchers, which use `scratch`).
     void* work = nullptr;

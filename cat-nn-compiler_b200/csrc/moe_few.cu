@@ -156,7 +156,8 @@ struct TcArgs {
     float* yp;        // [runs][T·k, hidden]: each pair's share of y from each run of rows, before its weight
     unsigned* taken;  // [T], then [T·k] weights: what the first kernel found (ALL)
     unsigned* count;  // [column tiles of hidden][T]: shares of a token that are there
-    int* status;
+    int* status;      // set to 1 when a wait ran out
+    long long patience;  // cycles after which a wait gives up; 0: the copying warps give up before their first tile
     int T, hidden, mid, E, k;
     int up_run, down_run;  // rows of a matrix that one CTA takes
     int counts;
@@ -455,8 +456,9 @@ template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct
     static_assert(ROOM % 1024 == 0 && MIN_STAGES >= 2, "two stages at least");
     static_assert(RED * 4 <= ROOM && (M == 1 && ALL ? 0 : PRE * W_BYTES + SCRATCH) <= ROOM,
                   "the parts, and routing beside the first stages, lie in the ring");
-    static_assert(1024 + ROOM + 2 * MAX_STAGES * 8 + MAX_T * (8 + 4 * MAX_E) <= SMEM_MAX, "smem()'s largest");
-    static size_t smem(int tokens, int k) { return 1024 + ROOM + 2 * MAX_STAGES * 8 + routes_bytes(tokens, k); }
+    static constexpr int BESIDE = 1024 + 2 * MAX_STAGES * 8 + 16;  // the ring's alignment, barriers, `stop`
+    static_assert(ROOM + BESIDE + MAX_T * (8 + 4 * MAX_E) <= SMEM_MAX, "smem()'s largest");
+    static size_t smem(int tokens, int k) { return ROOM + BESIDE + routes_bytes(tokens, k); }
 
     // fp32: a tile's tokens are split over 2^teams(n) teams of warps, G or fewer to each
     static __device__ __forceinline__ int teams(int n) {
@@ -468,6 +470,7 @@ template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct
 
     char* ring;
     uint64_t *full, *empty;
+    int* stop;  // not 0: a wait of this CTA ran out
     const CUtensorMap* w[2];
     int r0, r1, col0, iters;
 
@@ -476,7 +479,8 @@ template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct
         ring = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
         full = (uint64_t*)(ring + ROOM);
         empty = full + MAX_STAGES;
-        r.taken = (unsigned*)(empty + MAX_STAGES);
+        stop = (int*)(empty + MAX_STAGES);
+        r.taken = (unsigned*)(stop + 4);
         r.w = (float*)(r.taken + a.T);
         r.tok = (short*)(r.w + a.T * a.k);
         r.pair = r.tok + a.T;
@@ -491,6 +495,7 @@ template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct
                 tc::mbar_init(&full[s], 1 + 32);  // the weights' bytes, and the copying warp's lanes
                 tc::mbar_init(&empty[s], CW);
             }
+            *stop = 0;
             tc::fence_mbar_init();
         }
     }
@@ -508,12 +513,26 @@ template <typename T, bool ALL, int M, int NT, int BN_, int CW, int ROOM> struct
             for (int c = 0; c < BN; c += BOX)
                 tc::tma_load_3d(at + (m * BN + c) * BK * ES, w[m], col0 + c, r0 + it * BK, expert, &full[st]);
     }
+    // A lane's wait for a phase; after one of the CTA's ran out the others have next to no patience left. The loops
+    // go on all the same, with what is in the ring: a way out of them, which all lanes would have to agree on, cost 1.4
+    // us at 64 tokens (bf16) and 8 in fp32.
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const TcArgs& a) const {
+        if (tc::mbar_try_wait(tc::smem_u32(bar), parity)) return true;
+        return tc::mbar_wait(bar, parity, stop, 1, *(volatile int*)stop ? 0 : a.patience, false);
+    }
+    // After a wait ran out, by the copying warp: let the last of the tiles that it asked for land in each of the stages
+    // (whose sums come to lie there), which is a matter of microseconds, and leave word.
+    __device__ __forceinline__ void settle(const TcArgs& a, int asked, int stages) const {
+        for (int st = 0; st < stages && st < asked; ++st)
+            if (!tc::mbar_wait(&full[st], (asked - 1 - st) / stages & 1, stop, 1, 4000000000ll, false)) break;
+        atomicExch(a.status, 1);
+    }
     // An expert that no token takes: let what was fetched land, then leave.
     __device__ __forceinline__ void drain(const TcArgs& a) const {
         if (threadIdx.x >= CW * 32)
             for (int it = 0; it < PRE && it < iters; ++it) {
                 tc::mbar_arrive(&full[it]);
-                tc::mbar_wait(&full[it], 0, a.status, 4, 4000000000ll, false);
+                tc::mbar_wait(&full[it], 0, a.status, 1, 4000000000ll, false);
             }
     }
 };
@@ -547,6 +566,7 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
     // fp32: this warp's tokens [t0, t0 + G), of which `per` are its own, and its share of a tile's rows
     const int teams = S::teams(r.n), kg32 = warp >> teams;
     const int per = (((r.n + (1 << teams) - 1) >> teams) + 3) & ~3, t0 = (warp & (1 << teams) - 1) * per;
+    int asked = 0;  // tiles that the copying warp asked for
     if (warp == CW) {
         auto tokens = [&](int it, int st) {
             constexpr int P = BK / PIECE<T>;  // 16-byte pieces of a row
@@ -558,18 +578,20 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
                 tc::cp_async16(at + row * XPITCH<T> + c * 16, rows + (i64)idx[row] * len + (on ? k0 + c * PIECE<T> : 0), on);
             }
             tc::cp_async_arrive(&s.full[st]);
+            ++asked;
         };
+        bool lost = a.patience == 0;  // a wait of this lane's ran out: it asks for nothing more
         // weights first: they wait for nobody
-        if (lane == 0)
+        if (lane == 0 && !lost)
             for (int it = S::PRE; it < iters && it < stages; ++it) s.weights(it, it, r.expert);
         __syncwarp();
         wait();
-        for (int it = 0; it < iters && it < stages; ++it) tokens(it, it);
+        for (int it = 0; it < iters && it < (lost ? S::PRE : stages); ++it) tokens(it, it);
         for (int it = stages, st = 0, ph = 0; it < iters; ++it) {
-            tc::mbar_wait(&s.empty[st], ph, a.status, 4, 4000000000ll, false);
-            if (lane == 0) s.weights(it, st, r.expert);
+            lost = lost || !s.wait(&s.empty[st], ph, a);
+            if (lane == 0 && !lost) s.weights(it, st, r.expert);
             __syncwarp();
-            tokens(it, st);
+            if (!lost) tokens(it, st);
             if (++st == stages) st = 0, ph ^= 1;
         }
     } else if constexpr (F32) {
@@ -577,7 +599,7 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
         const int share = BK / CW << teams, mine = min(per, r.n - t0);
         for (int it = 0, st = 0, ph = 0; it < iters; ++it) {
             const int kk = min(BK, s.r1 - s.r0 - it * BK), k1 = min(kk, (kg32 + 1) * share);  // kk is a multiple of 4
-            tc::mbar_wait(&s.full[st], ph, a.status, 4, 4000000000ll, false);
+            s.wait(&s.full[st], ph, a);
             const float* wt = (const float*)(s.ring + st * S::W_BYTES) + lane;
             const char* xt = xring + st * xbytes + t0 * XPITCH<T>;
 #pragma unroll 1
@@ -615,7 +637,7 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
         const uint32_t wcol = wm / (S::BOX / 16) * (BK * S::BOX * 2), chunk = wm % (S::BOX / 16) * 2 + mid8;
         for (int it = 0, st = 0, ph = 0; it < iters; ++it) {
             const int kk = min(BK, s.r1 - s.r0 - it * BK);
-            tc::mbar_wait(&s.full[st], ph, a.status, 4, 4000000000ll, false);
+            s.wait(&s.full[st], ph, a);
             const uint32_t wb = tc::smem_u32(s.ring + st * S::W_BYTES) + wcol, xb = tc::smem_u32(xring + st * xbytes);
 #pragma unroll
             for (int k2 = 0; k2 < BK; k2 += 32 * S::KG) {
@@ -648,8 +670,14 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
             if (++st == stages) st = 0, ph ^= 1;
         }
     }
-    __syncthreads();  // every tile of the ring has landed and been read
+    __syncthreads();  // every tile of the ring has landed and been read, or a wait ran out
+    const bool stopped = *(volatile int*)s.stop != 0;  // then the sums are NaN
+    if (stopped) {
+        if (warp == CW) s.settle(a, asked, stages);
+        __syncthreads();
+    }
     if (warp == CW) return;
+    const float nan = __uint_as_float(0x7fc00000u);
     if constexpr (F32) {
         const int rows = S::red_rows(r.n);
 #pragma unroll
@@ -658,7 +686,7 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
 #pragma unroll
                 for (int c = 0; c < COLS; ++c)
                     ((float*)s.ring)[((kg32 * M + c / (BN / 32)) * rows + t0 + t) * S::RED_PITCH + c % (BN / 32) * 32 + lane] =
-                        sum2(sum[t][c]);
+                        stopped ? nan : sum2(sum[t][c]);
     } else {
         const int wm = warp % (BN / 16), kg = warp / (BN / 16);
         float* red = (float*)s.ring + kg * M * NT * 8 * S::RED_PITCH + wm * 16 + (lane >> 2) + (lane & 3) * 2 * S::RED_PITCH;
@@ -669,7 +697,7 @@ __device__ __forceinline__ void product(const Tc<T, ALL, M, NT, BN, CW, ROOM>& s
                 if (j >= nte) break;
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    red[(m * NT * 8 + j * 8 + (u & 1)) * S::RED_PITCH + (u >> 1) * 8] = acc[m][j][u];
+                    red[(m * NT * 8 + j * 8 + (u & 1)) * S::RED_PITCH + (u >> 1) * 8] = stopped ? nan : acc[m][j][u];
             }
     }
 }
@@ -979,8 +1007,8 @@ static void moe_few_tc(Context* c, const void* x, const void* gate, const void* 
     const Layout l = layout<Ty>(c, T, hidden, mid, E, k);
     char* at = (char*)work;
     run_tc<Ty>(c,
-               {x, gate, work, y, (float*)(at + l.yp), (unsigned*)(at + l.taken), (unsigned*)(at + l.count), c->status, (int)T,
-                (int)hidden, (int)mid, (int)E, (int)k, 0, 0, 0},
+               {x, gate, work, y, (float*)(at + l.yp), (unsigned*)(at + l.taken), (unsigned*)(at + l.count),
+                c->status + FEW_STATUS_SLOT, c->few_patience, (int)T, (int)hidden, (int)mid, (int)E, (int)k, 0, 0, 0},
                w1, w3, w2);
 }
 

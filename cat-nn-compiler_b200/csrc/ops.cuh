@@ -227,6 +227,7 @@ void paged_attention(Context* c, const void* q, i64 q_stride, const void* kc, co
                      i64 max_pages, i64 window, int dtype, void* work, int* err);
 
 // ---- a MoE layer for a few tokens (moe_few.cu)
+constexpr int FEW_STATUS_SLOT = 16;  // not 0: a wait of one of its kernels ran out
 size_t moe_few_workspace(Context* c, i64 T, i64 hidden, i64 mid, i64 E, i64 k, int dtype);
 void moe_few(Context* c, const void* x, const void* gate, const void* w1, const void* w3, const void* w2, void* y, i64 T,
              i64 hidden, i64 mid, i64 E, i64 k, int dtype, void* work);

@@ -360,6 +360,14 @@ int catnn_moe_few_workspace(catnn_ctx* ctx, int64_t T, int64_t hidden, int64_t m
 int catnn_moe_few_fwd(catnn_ctx* ctx, const void* x, const void* gate, const void* w1s, const void* w3s,
                       const void* w2s, void* y, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k,
                       int dtype, void* workspace, size_t workspace_bytes);
+/* The kernels' waits for their own copies are bounded (default 2 s). Where one
+ * runs out the rows of y that it reaches are NaN, and the next
+ * catnn_moe_few_check, which synchronizes, returns CATNN_ERR_TIMEOUT and
+ * clears it; no other call looks at it. 0 ms: the
+ * kernels give up before they ask for their tiles, for tests of the failure
+ * path. A captured call keeps the bound that it was captured with. */
+int catnn_moe_few_set_timeout_ms(catnn_ctx* ctx, int64_t ms);
+int catnn_moe_few_check(catnn_ctx* ctx);
 
 /* ------------------------------------------------------------ optimizers */
 /* p -= lr·g (Sgd::put, crates/catnn-core/src/lens/optim.rs:32). fp32

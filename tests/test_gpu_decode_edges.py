@@ -14,7 +14,7 @@ from test_gpu_decode import (BF, EPS, F32, U, check_attention, check_moe, gather
 pytestmark = pytest.mark.gpu
 
 from catnn_b200 import _lib, ops  # noqa: E402
-from catnn_b200.errors import ShapeMismatch  # noqa: E402
+from catnn_b200.errors import DeviceTimeout, InvalidArgument, ShapeMismatch  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -177,3 +177,33 @@ def test_moe_few_experts_shut_off(t, hid, mid, e, dtype):
         y2 = ops.moe_few(bad, gate, w1, w3, w2, 2)
         others = [i for i in range(t) if i != 1]
         assert torch.equal(y2[others], y[others]) and not torch.isfinite(y2[1]).all()
+
+
+# ------------------------------------------------------------------ waits that run out
+@pytest.mark.parametrize("dtype,t,hid,mid,e", [(BF, 1, 1024, 1024, 8), (BF, 8, 512, 1024, 32), (BF, 64, 1024, 3584, 8),
+                                               (F32, 3, 256, 512, 8), (F32, 12, 1024, 1024, 8), (F32, 50, 1024, 3584, 4)])
+def test_moe_few_reports_a_wait_that_runs_out(dtype, t, hid, mid, e):
+    """With no patience at all the kernels give up before their tiles are there:
+    their rows are NaN, the check says so once, and neither another operator nor
+    the next call is the worse for it."""
+    args = moe_inputs(75, dtype, t, hid, mid, e)
+    good = ops.moe_few(*args, 2, check=True)
+    a, b = rand(gen(76), 300, 256, dtype=BF), rand(gen(77), 256, 300, dtype=BF)
+    product = ops.gemm(a, b)
+    h = ops.context(args[0].device).bind()
+    _lib.call("catnn_moe_few_set_timeout_ms", h, 0)
+    try:
+        y = ops.moe_few(*args, 2)
+        assert torch.equal(ops.gemm(a, b), product)
+        assert torch.isnan(y).any() and bool((torch.isnan(y) | (y == good)).all())
+        with pytest.raises(DeviceTimeout):
+            _lib.call("catnn_moe_few_check", h)
+        _lib.call("catnn_moe_few_check", h)
+        with pytest.raises(DeviceTimeout):
+            ops.moe_few(*args, 2, check=True)
+    finally:
+        _lib.call("catnn_moe_few_set_timeout_ms", h, 2000)
+    assert torch.equal(ops.moe_few(*args, 2, check=True), good)
+    for ms in (-1, 2 ** 40):
+        with pytest.raises(InvalidArgument):
+            _lib.call("catnn_moe_few_set_timeout_ms", h, ms)

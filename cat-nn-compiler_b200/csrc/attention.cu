@@ -219,12 +219,12 @@ __global__ void __launch_bounds__(256) k_rope(T* __restrict__ x, const float2* _
 }
 
 const float2* rope_table(Context* c, i64 s, i64 hd, double theta) {
+    if (!c->rope_captured) c->rope_captured = c->rope_tab && c->capturing();
     if (c->rope_tab && c->rope_s == s && c->rope_hd == hd && c->rope_theta == theta) return (const float2*)c->rope_tab;
-    if (c->rope_tab) {
-        CUDA_OK(cudaStreamSynchronize(c->stream));
-        CUDA_OK(cudaFree(c->rope_tab));
-        c->rope_tab = nullptr;
-    }
+    void* old = c->rope_tab;
+    c->rope_tab = nullptr;
+    c->let_go(old, c->rope_captured);
+    c->rope_captured = false;
     i64 n = s * (hd / 2);
     CUDA_OK(cudaMalloc(&c->rope_tab, (size_t)(n > 0 ? n : 1) * sizeof(float2)));
     int grid = (int)((n + 255) / 256);

@@ -9,6 +9,7 @@
 #include <stdexcept>
 #include <initializer_list>
 #include <string>
+#include <vector>
 
 #include "../../include/catnn_b200.h"
 
@@ -68,6 +69,12 @@ struct Context {
     size_t work_bytes = 0;
     void* scratch_for(size_t bytes);
     void* work_for(size_t bytes);
+    // A captured graph holds the arenas and the table that its calls were given:
+    // what a capture has seen is kept until the context ends.
+    bool arenas_captured = false, rope_captured = false;
+    std::vector<void*> outgrown;
+    bool capturing() const;             // whether the stream is
+    void let_go(void* p, bool keep);  // keeps p, or frees it once the stream is done
 };
 
 // Carves aligned sub-buffers out of one arena allocation.

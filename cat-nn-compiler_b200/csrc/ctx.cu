@@ -23,35 +23,42 @@ int take_status(Context* c, int slot) {
 static int g_live_ctx[64] = {0};
 static std::mutex g_live_ctx_mu;
 
-void* Context::scratch_for(size_t bytes) {
-    if (bytes <= scratch_bytes) return scratch;
-    // Grow-only: the stream must not still be reading the old buffer.
-    if (scratch) {
-        CUDA_OK(cudaStreamSynchronize(stream));
-        CUDA_OK(cudaFree(scratch));
-        scratch = nullptr;
-        scratch_bytes = 0;
-    }
-    size_t b = bytes < (1u << 20) ? (1u << 20) : bytes;
-    b = (b + 255) & ~(size_t)255;
-    CUDA_OK(cudaMalloc(&scratch, b));
-    scratch_bytes = b;
-    return scratch;
+bool Context::capturing() const {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    CUDA_OK(cudaStreamIsCapturing(stream, &st));
+    return st != cudaStreamCaptureStatusNone;
 }
 
-void* Context::work_for(size_t bytes) {
-    if (bytes <= work_bytes) return work;
-    if (work) {
-        CUDA_OK(cudaStreamSynchronize(stream));
-        CUDA_OK(cudaFree(work));
-        work = nullptr;
-        work_bytes = 0;
+void Context::let_go(void* p, bool keep) {
+    if (!p) return;
+    if (keep) {
+        outgrown.push_back(p);
+        return;
     }
-    size_t b = (bytes + 255) & ~(size_t)255;
-    CUDA_OK(cudaMalloc(&work, b));
-    work_bytes = b;
-    return work;
+    CUDA_OK(cudaStreamSynchronize(stream));
+    CUDA_OK(cudaFree(p));
 }
+
+// Grow-only. After a capture the next size is at least twice as large, so that
+// all that was outgrown stays below what is in use.
+static void* grown(Context* c, void*& at, size_t& have, size_t bytes, size_t least) {
+    if (!c->arenas_captured) c->arenas_captured = c->capturing();
+    if (bytes <= have) return at;
+    size_t b = bytes < least ? least : bytes;
+    if (c->arenas_captured && b < 2 * have) b = 2 * have;
+    b = (b + 255) & ~(size_t)255;
+    void* old = at;
+    at = nullptr;
+    have = 0;
+    c->let_go(old, c->arenas_captured);
+    CUDA_OK(cudaMalloc(&at, b));
+    have = b;
+    return at;
+}
+
+void* Context::scratch_for(size_t bytes) { return grown(this, scratch, scratch_bytes, bytes, (size_t)1 << 20); }
+
+void* Context::work_for(size_t bytes) { return grown(this, work, work_bytes, bytes, 0); }
 
 // FNV-1a over f32 bit patterns is inherently sequential; a single thread
 // walks the tensor (it is a debugging/sheaf checksum, not a hot kernel).
@@ -123,6 +130,7 @@ int catnn_ctx_destroy(catnn_ctx* h) {
     if (h->c.tc_sched) cudaFree(h->c.tc_sched);
     if (h->c.rope_tab) cudaFree(h->c.rope_tab);
     if (h->c.work) cudaFree(h->c.work);
+    for (void* p : h->c.outgrown) cudaFree(p);
     {
         std::lock_guard<std::mutex> lock(g_live_ctx_mu);
         if (--g_live_ctx[h->c.device] == 0) xent_noalloc_forget(h->c.device);

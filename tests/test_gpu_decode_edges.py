@@ -8,12 +8,13 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode import (BF, EPS, F32, U, check_attention, check_moe, gather, gen, inv_rms, make_cache, moe_inputs,
+from test_gpu_decode import (BF, EPS, F32, Layer, U, check_attention, check_moe, gather, gen, inv_rms, make_cache, moe_inputs,
                              own_rounding, pair_size, qk_inputs, rand, turn, u, within)
 
 pytestmark = pytest.mark.gpu
 
 from catnn_b200 import _lib, ops  # noqa: E402
+from catnn_b200.train import MoeConfig, MoeTrainer, init_params  # noqa: E402
 from catnn_b200.errors import DeviceTimeout, InvalidArgument, ShapeMismatch  # noqa: E402
 
 
@@ -207,3 +208,94 @@ def test_moe_few_reports_a_wait_that_runs_out(dtype, t, hid, mid, e):
     for ms in (-1, 2 ** 40):
         with pytest.raises(InvalidArgument):
             _lib.call("catnn_moe_few_set_timeout_ms", h, ms)
+
+
+# ------------------------------------------------------------------ captured calls and what the context keeps
+def outgrow(dtype):
+    """Calls whose split sums and temporaries are larger than all before them."""
+    for k in (2 ** 14, 2 ** 16):
+        a = torch.ones(1024, k, dtype=BF, device="cuda")
+        assert float(ops.gemm(a, a, trans_b=True)[0, 0]) == k
+    big = moe_inputs(81, dtype, 3000, 256, 512, 8)
+    return ops.moe(*big, 2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_a_captured_layer_outlives_larger_calls(dtype):
+    """A whole layer of a decoding step as a graph, products with split sums
+    among it, replayed after eager calls that outgrow the context's memory."""
+    layer = Layer(dtype, hid=1024, h=16, hkv=4, mid=1024, seed=82)
+    g = gen(83)
+    kc, vc, table, lens = make_cache(g, dtype, [60] * 5, 4, 64, 16)
+    lens[:] = torch.arange(5, device="cuda") * 7 + 3
+    x = rand(g, 5, 1024, dtype=dtype)
+    layer.step(x, kc, vc, table, lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        layer.step(x, kc, vc, table, lens)
+        with torch.cuda.graph(graph, stream=side):
+            y = layer.step(x, kc, vc, table, lens)
+    torch.cuda.current_stream().wait_stream(side)
+    for r in range(4):
+        if r:
+            assert torch.isfinite(outgrow(dtype).float()).all()
+            torch.cuda.synchronize()
+        x.copy_(rand(g, 5, 1024, dtype=dtype))
+        lens += 1
+        graph.replay()
+        got = (y.clone(), kc.clone(), vc.clone())
+        want = (layer.step(x, kc, vc, table, lens), kc, vc)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), r
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_a_captured_rotation_keeps_its_angles(dtype):
+    """A captured rope after eager calls of other lengths and bases."""
+    g = gen(84)
+    x = rand(g, 2, 100, 4, 64, dtype=dtype)
+    y = torch.empty_like(x)
+    want = ops.rope(x.clone(), 1e4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y.copy_(x)
+        ops.rope(y, 1e4)
+    for s, theta in ((100, 1e6), (3000, 1e4), (7, 1e4), (100, 1e5)):
+        ops.rope(rand(g, 1, s, 4, 64, dtype=dtype), theta)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    long = rand(g, 1, 4096, 4, 64, dtype=dtype)
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(40):  # tables that no capture holds are not kept
+        ops.rope(x, 1e5)
+        ops.rope(long, 1e4)
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] < 32 * 2 ** 20
+
+
+def test_a_captured_training_step_outlives_larger_calls():
+    """The trainer's graph, replayed after eager calls that outgrow the memory
+    and change the table that its capture was given."""
+    cfg = MoeConfig.make(1024, 256, 512, 2, 4, 4, 8, 2, batch=2, seq=128, rope_theta=1e6, dtype=BF, optimizer="adam", lr=1e-3)
+    params = init_params(cfg, 85)
+    tok = torch.randint(0, 1024, (256,), generator=gen(85), device="cuda", dtype=torch.int32)
+    a, b = MoeTrainer(cfg), MoeTrainer(cfg)
+    a.set_params(params)
+    b.set_params(params)
+    b.set_graphs(True)
+    la, lb = torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda")
+    for i in range(6):
+        a.step(tok, update=True, loss_out=la)
+        b.step(tok, update=True, loss_out=lb)
+        torch.cuda.synchronize()
+        assert torch.equal(la, lb), i
+        if i > 2:  # captured by now
+            outgrow(BF)
+            ops.rope(rand(gen(i), 1, 50 + i, 4, 64, dtype=BF), 1e4)
+    assert torch.equal(a.params(), b.params())
+    a.close()
+    b.close()

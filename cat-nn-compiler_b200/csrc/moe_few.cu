@@ -973,6 +973,8 @@ template <typename T> static void run_tc(Context* c, TcArgs a, const void* w1, c
         using P = decltype(shape);
         using U = Tc<T, P::ALL, 2, P::NT, P::BU, P::CU, P::RU>;
         using D = Tc<T, P::ALL, 1, P::NT, P::BD, P::CD, P::RD>;
+        // found first, the experts are found twice, and by the same sums: their order goes by the number of warps
+        static_assert(P::ALL || P::CU == P::CD, "both kernels must choose the same experts to the last bit");
         const int dt = sizeof(T) == 4 ? CATNN_F32 : CATNN_BF16;
         const CUtensorMap m1 = tma_map_stack(w1, a.E, a.hidden, a.mid, dt, U::BOX, BK);
         const CUtensorMap m3 = tma_map_stack(w3, a.E, a.hidden, a.mid, dt, U::BOX, BK);

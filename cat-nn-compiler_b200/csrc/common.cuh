@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <stdexcept>
 #include <initializer_list>
+#include <set>
 #include <string>
 #include <vector>
 
@@ -61,6 +62,9 @@ struct Context {
     double turns[128] = {0.0};
     i64 turns_hd = 0;
     double turns_theta = 0.0;
+    // Kernels whose limit of shared memory was raised (it holds for the device
+    // from then on; entered once that has succeeded).
+    std::set<const void*> raised;
     // Cycles after which a wait of the MoE for a few tokens gives up (moe_few.cu); about 2 s.
     long long few_patience = 4000000000ll;
     // Grow-only arena for composite ops (several temporaries held across

@@ -15,9 +15,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <mutex>
-#include <set>
-#include <utility>
 
 #include "ops.cuh"
 #include "tc_prims.cuh"
@@ -857,16 +854,11 @@ static int runs_of(Context* c, i64 tiles, i64 rows, int per_sm) {
 
 template <typename Kern, typename... A>
 static void launch(Context* c, Kern k, int threads, dim3 grid, dim3 cluster, size_t smem, bool dependent, const A&... args) {
-    // a function's limit on one device holds from then on; `Kern` is the same type for several kernels
-    static std::mutex mu;
-    static std::set<std::pair<const void*, int>> raised;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (raised.insert({(const void*)k, c->device}).second) {
-            CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
-            // all of the SM's memory as shared: the second kernel's CTAs come to SMs that the first still holds
-            CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        }
+    if (!c->raised.count((const void*)k)) {
+        CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
+        // all of the SM's memory as shared: the second kernel's CTAs come to SMs that the first still holds
+        CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+        c->raised.insert((const void*)k);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;

@@ -20,8 +20,6 @@
 // of 64: 6.5 us; 49.5 K positions of 2 kv heads of 64, fp32, 51 MB: 21.0 us.
 #include <algorithm>
 #include <climits>
-#include <mutex>
-#include <set>
 
 #include "ops.cuh"
 #include "paged_place.cuh"
@@ -754,12 +752,9 @@ static Layout layout(Context* c, i64 h, i64 hkv, i64 hd, int dtype) {
 }
 
 template <typename Kern> static void launch(Context* c, Kern k, int grid, int threads, size_t smem, const Args& a) {
-    static std::mutex mu;
-    static std::set<std::pair<const void*, int>> raised;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (raised.insert({(const void*)k, c->device}).second)
-            CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (!c->raised.count((const void*)k)) {
+        CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        c->raised.insert((const void*)k);
     }
     k<<<grid, threads, smem, c->stream>>>(a);
     launched(c);

@@ -14,7 +14,7 @@ from test_gpu_decode import (BF, EPS, F32, Layer, U, check_attention, check_moe,
 pytestmark = pytest.mark.gpu
 
 from catnn_b200 import _lib, ops  # noqa: E402
-from catnn_b200.train import MoeConfig, MoeTrainer, init_params  # noqa: E402
+from catnn_b200.train import MoeConfig, MoeTrainer, init_params, packed_layout  # noqa: E402
 from catnn_b200.errors import DeviceTimeout, InvalidArgument, ShapeMismatch  # noqa: E402
 
 
@@ -299,3 +299,74 @@ def test_a_captured_training_step_outlives_larger_calls():
     assert torch.equal(a.params(), b.params())
     a.close()
     b.close()
+
+
+# ------------------------------------------------------------------ a trained decoder
+def decoder_weights(trainer):
+    """The weights of a trainer's packed vector, as the operators take them."""
+    cfg, at, p = trainer.cfg, packed_layout(trainer.cfg), trainer.params()
+    h, f, e, hd = cfg.hidden, cfg.mid, cfg.experts, cfg.hidden // cfg.heads
+
+    def take(start, *shape):
+        return p[start:start + math.prod(shape)].view(*shape)
+    layers = []
+    for i in range(cfg.layers):
+        base = at["layer0"] + i * at["layer_stride"]
+        w = {n: take(base + at[n], *s) for n, s in (
+            ("rms_attn", (h,)), ("wq", (h, h)), ("wk", (h, cfg.kv_heads * hd)), ("wv", (h, cfg.kv_heads * hd)), ("wo", (h, h)),
+            ("rms_moe", (h,)), ("gate", (h, e)), ("w1", (e, h, f)), ("w3", (e, h, f)), ("w2", (e, f, h)))}
+        w = {n: t if n.startswith("rms") or cfg.dtype == 0 else t.to(BF) for n, t in w.items()}
+        w["wqkv"] = torch.cat((w["wq"], w["wk"], w["wv"]), 1).contiguous()
+        layers.append({n: t.contiguous() for n, t in w.items()})
+    return take(0, cfg.vocab, h), layers, take(at["final_norm"], h), take(at["lm_head"], cfg.vocab, h)
+
+
+def test_decoding_with_a_trainers_weights():
+    """Prompts in one go, then token by token, against the activations of the
+    trainer's own pass over the whole sequences."""
+    b, s, prompt, page = 3, 40, 23, 16
+    cfg = MoeConfig.make(512, 256, 512, 2, 4, 2, 8, 2, batch=b, seq=s, dtype=F32, optimizer="adam", lr=1e-3)
+    tr = MoeTrainer(cfg)
+    tr.set_params(init_params(cfg, 86, std=0.05))
+    tok = torch.randint(0, 512, (b, s), generator=gen(86), device="cuda", dtype=torch.int32)
+    for _ in range(3):
+        tr.step(tok.view(-1), update=True)
+    tr.step(tok.view(-1), update=False)
+    want = tr.activation("xf").view(b, s, 256).double()
+    for i in range(2):  # no choice of experts may hang on the last bits
+        sel = tr.activation("router_logits", i).sort(-1, descending=True)[0]
+        assert float((sel[:, 1] - sel[:, 2]).min()) > 1e-5, "the test's inputs: choose another seed"
+    embed, layers, norm, _ = decoder_weights(tr)
+    h, hkv, hd, eps, theta = 4, 2, 64, cfg.rms_eps, cfg.rope_theta
+    pools = [(torch.empty(9, hkv, page, hd, device="cuda"), torch.empty(9, hkv, page, hd, device="cuda")) for _ in layers]
+    table = torch.randperm(9, generator=gen(87), device="cuda").int().view(b, 3).contiguous()
+    lens = torch.full((b,), prompt, dtype=torch.int32, device="cuda")
+    cu = torch.arange(b + 1, device="cuda", dtype=torch.int32) * prompt
+
+    def forward(x, cu=None):
+        for w, (kc, vc) in zip(layers, pools):
+            q, k, v = (t.unflatten(-1, (-1, hd)) for t in ops.gemm(ops.rmsnorm(x, w["rms_attn"], eps), w["wqkv"]).split(
+                [h * hd, hkv * hd, hkv * hd], -1))
+            q = ops.kv_append(q, k, v, kc, vc, table, lens, theta, cu_tokens=cu, check=True)
+            if cu is None:
+                o, _ = ops.paged_attention(q, kc, vc, table, lens, check=True)
+            else:  # prompts of one length: their keys rotated once more, for the attention of whole sequences
+                k, v = (t.reshape(b, prompt, hkv, hd).contiguous() for t in (k, v))
+                o, _ = ops.attention_core(q.view(b, prompt, h, hd), ops.rope(k, theta), v)
+                o = o.view(b * prompt, h * hd)
+            x = ops.add(x, ops.gemm(o, w["wo"]))
+            y = ops.rmsnorm(x, w["rms_moe"], eps)
+            moe = ops.moe_few(y, *(w[n] for n in ("gate", "w1", "w3", "w2")), 2) if len(y) <= 64 else \
+                ops.moe(y, *(w[n] for n in ("gate", "w1", "w3", "w2")), 2)
+            x = ops.add(x, moe)
+        return ops.rmsnorm(x, norm, eps)
+
+    def close(got, ref, what):
+        # as test_decoding_a_layer_matches_whole_sequences: 2e-5 a layer, once more for the final norm
+        rel = float((got.double() - ref).norm() / ref.norm())
+        assert rel <= 6e-5, (what, rel)
+    close(forward(embed[tok[:, :prompt].reshape(-1).long()], cu).view(b, prompt, 256), want[:, :prompt], "prompts")
+    for t in range(prompt, s):
+        lens += 1
+        close(forward(embed[tok[:, t].long()]), want[:, t], t)
+    tr.close()

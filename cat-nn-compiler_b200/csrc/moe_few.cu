@@ -214,17 +214,18 @@ __device__ __forceinline__ unsigned choose(float l, int E, int k, int lane, floa
 // fp32 logits of token t by a warp, lane e holding expert e's: an infinite
 // value, or one that TF32 rounds to infinity, leaves NaN as its lower half,
 // so logits that came out NaN are added up again from the values as they are
-// (an expert shut off by -inf then has the logit -inf), unless the token's own
-// row has a NaN, such as the stale rows of a padded batch.
+// (an expert shut off by -inf then has the logit -inf). Not where the token's
+// own row has a NaN or an infinity, as stale rows of a padded batch may: then
+// every logit is infinite or NaN, and the weights are NaN whichever are chosen.
 __device__ __forceinline__ float exact_where_nan(const TcArgs& a, int t, float l) {
     const int lane = threadIdx.x & 31;
     unsigned left = __ballot_sync(0xffffffffu, l != l);
     if (left == 0) return l;
     const float* x = (const float*)a.x + (i64)t * a.hidden;
-    bool nan = false;
+    bool finite = true;
 #pragma unroll 8
-    for (int i = lane; i < a.hidden; i += 32) nan |= x[i] != x[i];
-    if (__any_sync(0xffffffffu, nan)) return l;
+    for (int i = lane; i < a.hidden; i += 32) finite &= fabsf(x[i]) < INFINITY;
+    if (!__all_sync(0xffffffffu, finite)) return l;
     for (; left; left &= left - 1) {
         const int e = __ffs(left) - 1;
         float s = 0.f;

@@ -180,6 +180,19 @@ def test_moe_few_experts_shut_off(t, hid, mid, e, dtype):
         assert torch.equal(y2[others], y[others]) and not torch.isfinite(y2[1]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("t,hid,mid,e,k", [(3, 128, 128, 8, 1), (5, 128, 136, 8, 2), (20, 136, 128, 32, 3), (4, 24, 40, 8, 2)])
+def test_moe_few_infinite_rows(t, hid, mid, e, k, dtype):
+    """A row with an infinity has infinite logits, whose softmax is NaN; so is
+    a row of NaN. Neither reaches another row."""
+    x, gate, w1, w3, w2 = moe_inputs(78 + hid, dtype, t, hid, mid, e)
+    y = ops.moe_few(x, gate, w1, w3, w2, k)
+    x[1, 7], x[2, 9], x[2, 11] = math.inf, -math.inf, math.nan
+    y2 = ops.moe_few(x, gate, w1, w3, w2, k)
+    others = [i for i in range(t) if i not in (1, 2)]
+    assert torch.isnan(y2[1:3]).all() and torch.equal(y2[others], y[others])
+
+
 # ------------------------------------------------------------------ waits that run out
 @pytest.mark.parametrize("dtype,t,hid,mid,e", [(BF, 1, 1024, 1024, 8), (BF, 8, 512, 1024, 32), (BF, 64, 1024, 3584, 8),
                                                (F32, 3, 256, 512, 8), (F32, 12, 1024, 1024, 8), (F32, 50, 1024, 3584, 4)])

@@ -18,6 +18,13 @@ F32, BF16, TF32 = 0, 1, 2
 ACT = {"none": 0, None: 0, "relu": 1, "gelu": 2}
 
 
+def _stream_of(device):
+    """The handle of torch's current stream, without the object round it where
+    torch offers that (a call's host side 2.0 -> 0.6 us)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
 class Context:
     """One libcatnn_b200 context per device (catnn_ctx_create)."""
 
@@ -30,8 +37,7 @@ class Context:
 
     def bind(self):
         # set on every call: another thread, or a caller of the C ABI, may have set another one since
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(s))
+        _lib.call("catnn_ctx_set_stream", self.handle, C.c_void_p(_stream_of(self.device)))
         return self.handle
 
     def workspace(self, name, *sizes):

@@ -103,3 +103,14 @@ def test_bind_sets_the_stream_every_time(monkeypatch):
         handle["stream"] = other  # behind the context's back
         ctx.bind()
         assert handle["stream"] == mine
+
+
+def test_the_stream_without_torchs_shortcut(monkeypatch):
+    from types import SimpleNamespace
+
+    import torch
+
+    from catnn_b200 import ops
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=7 + device))
+    assert ops._stream_of(1) == 8

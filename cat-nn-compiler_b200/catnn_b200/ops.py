@@ -726,8 +726,11 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, window=None, chec
 
 
 def moe_few(x, gate, w1s, w3s, w2s, top_k, check=False):
-    """moe() for at most 64 rows of x, in two kernels that read each chosen
-    expert's weights once; expert weights stacked [E, ...]. check=True
+    """moe() for at most 64 rows of x (more are refused: moe() takes them), in
+    two kernels that read each chosen expert's weights once; expert weights
+    stacked [E, ...]. That is for hidden and mid of at least 64, multiples of 8
+    (fp32: 4), and operands on 16-byte boundaries; other calls are computed by
+    kernels that take 1 ms and more where these take 20 to 170 us. check=True
     (synchronizing) reports a bounded wait that ran out, in this call or one
     since the last check, as a DeviceTimeout; its rows are NaN."""
     _same(x, gate, w1s, w3s, w2s)

@@ -7,11 +7,17 @@
 // stream; with few tokens the routing before the stream, the hand-over of h
 // and the last sum take as long again.
 //
-// Measured at hidden 1024, mid 3584, 8 experts, top 2: bf16 1 token 18.9 us
-// (44 MB of weights, 2.3 TB/s), 8 tokens 33.5, 64 tokens 46.8 (176 MB, 3.8
-// TB/s); fp32 1 token 28.9 (88 MB), 16 tokens 77, 64 tokens 167 (352 MB; the
-// FMAs of 16 tokens an expert, and 448 tiles on 296 places). 7 tokens, hidden
-// 256, mid 512, fp32: 12.5 us.
+// Measured at hidden 1024, mid 3584, 8 experts, top 2: bf16 1 token 19.0 us
+// (44 MB of weights, 2.3 TB/s), 8 tokens 33.9, 64 tokens 47.4 (176 MB, 3.7
+// TB/s); the block for many tokens takes 267, 310 and 319. fp32 1 token 29.2
+// (88 MB), 16 tokens 76, 64 tokens 168 (352 MB; the FMAs of 16 tokens an
+// expert, and 448 tiles on 296 places). 7 tokens, hidden 256, mid 512, fp32:
+// 12.7 us.
+//
+// That is for hidden and mid of 64 and more, multiples of 8 (fp32: 4), and
+// operands on 16-byte boundaries. For the rest k_up_any and k_down_any keep the
+// call whole, one thread to a column, with every token reading its experts'
+// weights for itself: 1.2 to 1.8 ms at hidden 1022, mid 3582.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -141,7 +147,8 @@ __global__ void __launch_bounds__(THREADS) k_down_any(const __grid_constant__ Ar
 // bounds it beside HBM is the rows of x, 16 bytes that all lanes read at once
 // cost the registers' port as much as 512: with one column to a lane 64 tokens
 // took 264 us in place of 167 (hidden 1024, mid 3584). Its logits are TF32 products all the same, of both halves of every
-// value (a 21-bit product, as exact as the fp32 sums that it goes into).
+// value without that of the two lower halves: a product is off by up to 7
+// half-steps of fp32, which a sum of many of them hides and a single one does not.
 constexpr int BK = 64;
 template <typename T> constexpr int XPITCH = BK * (int)sizeof(T) + 16;
 template <typename T> constexpr int PIECE = 16 / (int)sizeof(T);
@@ -755,7 +762,7 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
         const float* u = (const float*)&v[0];
         const float* g = (const float*)&v[1];
         float h[4];
-        // held in the type that the second product multiplies in
+        // held in the type that the second product multiplies in (bf16 rounds it by up to 2^-8, and takes __expf)
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[j] = u[j] / (1.f + (sizeof(T) == 4 ? expf(-u[j]) : __expf(-u[j]))) * g[j];
         stv<T, 4>((T*)a.h + (i64)r.pair[t] * a.mid + s.col0 + c, h);
@@ -851,8 +858,9 @@ __global__ void __launch_bounds__((CW + 1) * 32, PER_SM)
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // How many runs a matrix's rows are cut into (at most 8, a cluster): as many
-// as the SMs hold CTAs at once, of at least two tiles each; with all of them
-// resident they share the memory evenly and end together.
+// as the SMs hold CTAs at once, of at least two tiles each, so that all are
+// resident. Runs are whole tiles of 64 rows, so the last ones may be shorter,
+// or have none (1152 rows in 8 runs: six of 192); what such a CTA adds is zero.
 static int runs_of(Context* c, i64 tiles, i64 rows, int per_sm) {
     int s = 1;
     while (s < 8 && tiles * 2 * s <= (i64)c->sm_count * per_sm && rows / (2 * s) >= 2 * BK) s *= 2;

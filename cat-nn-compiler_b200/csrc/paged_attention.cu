@@ -17,7 +17,9 @@
 //
 // Measured: 64 sequences up to 6000, 16 query and 4 kv heads of 128, bf16, 388
 // MB of cache: 73 us (0.81 of the copy rate); one sequence of 2047, 16 heads
-// of 64: 6.5 us; 49.5 K positions of 2 kv heads of 64, fp32, 51 MB: 21.0 us.
+// of 64: 6.6 us; 49.5 K positions of 2 kv heads of 64, fp32, 51 MB: 22.0 us.
+// A warp that comes from one sequence to the next passes those of no length one
+// by one: four of 1000 among 64, 256 and 1024 take 13.9, 24 and 80 us.
 #include <algorithm>
 #include <climits>
 

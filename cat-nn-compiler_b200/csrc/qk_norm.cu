@@ -7,11 +7,15 @@
 //   forward  y = R(p)·(x·r·w)
 //   adjoint  g = R(p)ᵀ·dy, x̂ = x·r, dw = Σ_rows g·x̂,
 //            dx = r·(g·w − x̂·mean(g·w·x̂))
-// Every kernel reads its rows once and writes them once, so HBM bounds them,
-// and next to it the instructions per value. Measured, bf16: 16384 tokens of
-// 16 + 4 heads of 64 forward 17.0 us (4.9 TB/s, 0.75 of the copy rate), adjoint
-// 27.4 us (4.6 TB/s); append of 14087 tokens of 16 + 2 x 4 heads of 128 with
-// the norm 39.9 us (4.1 TB/s); one token 2.7 us, an append of 32 single ones 4.4.
+// Every kernel reads its rows once and writes them once, so HBM bounds them;
+// what holds them off its rate is latency at low occupancy: a warp asks for a
+// batch of rows, computes, stores, and only then asks for the next, and the
+// registers of a batch leave 16 to 24 warps an SM. (Instruction issue does not:
+// at four a cycle and SM it would take 9, 14 and 19 us of the times below.)
+// Measured, bf16: 16384 tokens of 16 + 4 heads of 64 forward 17.1 us (4.9 TB/s,
+// 0.75 of the copy rate), adjoint 27.3 us (4.6 TB/s); append of 14087 tokens of
+// 16 + 2 x 4 heads of 128 with the norm 39.7 us (4.1 TB/s); one token 2.7 us, an
+// append of 32 single ones 4.4.
 //
 // A row is held by the smallest power-of-two group of lanes that takes it in
 // 16-byte pieces (8 bf16 or 4 fp32 values a lane; hd 80 and 96 leave lanes
@@ -74,8 +78,8 @@ template <int LPH> __device__ __forceinline__ float group_sum(float v) {
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 
 // Two floats in one register pair, for the instructions that work on both.
-// What bounds these kernels next to HBM is the number of instructions, so a
-// lane's values are taken two pairs at a time: X0 = the first elements of
+// They shorten what a warp does between its loads (54 -> 30 us in the adjoint):
+// a lane's values are taken two pairs at a time: X0 = the first elements of
 // pairs i and i + 1, X1 = their second elements.
 using namespace tc::pairs;
 

@@ -288,7 +288,10 @@ int catnn_moe_bwd(catnn_ctx* ctx, const void* x, const void* gate, const void* w
  * 256-byte aligned, at least the bytes its _workspace function returns; its
  * contents do not matter and it is free again once the call's work is done),
  * so that they allocate nothing, synchronize with nothing unless check != 0,
- * can be captured, and share nothing with calls on other streams. */
+ * can be captured, and share nothing with calls on other streams (a checked
+ * call uses a status word of the context). The products and norms between
+ * them may use the context's own memory: a call that is to be captured runs
+ * once before, and that memory is kept while the context lives. */
 
 /* q' = R(pos)·rmsnorm(q; wq), k' = R(pos)·rmsnorm(k; wk) for each head of
  * q [b,s,n_heads,hd] and k [b,s,n_kv,hd] (moe.rs:17 over hd, then moe.rs:47):
@@ -349,10 +352,13 @@ int catnn_paged_attention_fwd(catnn_ctx* ctx, const void* q, int64_t q_stride, c
                               int64_t page_size, int64_t max_pages, int64_t window, int dtype, void* workspace,
                               size_t workspace_bytes, int check);
 
-/* catnn_moe_fwd for at most CATNN_MOE_FEW_MAX_TOKENS rows of x: the same
- * block (router ties to the lower index, E <= 32) in two kernels that read
- * each chosen expert's weights once, with no padding of experts to 128 rows.
- * y must not overlap x. The second kernel starts beside the first (programmatic
+/* catnn_moe_fwd for at most CATNN_MOE_FEW_MAX_TOKENS rows of x (more are
+ * refused: catnn_moe_fwd takes them): the same block (router ties to the lower
+ * index, E <= 32) in two kernels that read each chosen expert's weights once,
+ * with no padding of experts to 128 rows. That needs hidden and mid of at least
+ * 64, multiples of 8 (fp32: 4), and all six operands on 16-byte boundaries;
+ * anything else is computed too, by kernels that read the weights once for
+ * every token (1 ms and more where the others take 20 to 170 us). y must not overlap x. The second kernel starts beside the first (programmatic
  * dependent launch), which a stream's other work does not notice. */
 #define CATNN_MOE_FEW_MAX_TOKENS 64
 int catnn_moe_few_workspace(catnn_ctx* ctx, int64_t T, int64_t hidden, int64_t mid, int64_t E, int64_t k, int dtype,

@@ -39,19 +39,26 @@ void Context::let_go(void* p, bool keep) {
     CUDA_OK(cudaFree(p));
 }
 
-// Grow-only. After a capture the next size is at least twice as large, so that
-// all that was outgrown stays below what is in use.
+// Grow-only. After a capture the next size is twice as large where the device
+// has that much, so that all that was outgrown stays below what is in use.
 static void* grown(Context* c, void*& at, size_t& have, size_t bytes, size_t least) {
     if (!c->arenas_captured) c->arenas_captured = c->capturing();
     if (bytes <= have) return at;
-    size_t b = bytes < least ? least : bytes;
-    if (c->arenas_captured && b < 2 * have) b = 2 * have;
-    b = (b + 255) & ~(size_t)255;
+    const auto rounded = [](size_t v) { return (v + 255) & ~(size_t)255; };
+    const size_t need = rounded(bytes < least ? least : bytes);
+    size_t b = c->arenas_captured && need < 2 * have ? rounded(2 * have) : need;
     void* old = at;
     at = nullptr;
     have = 0;
     c->let_go(old, c->arenas_captured);
-    CUDA_OK(cudaMalloc(&at, b));
+    cudaError_t e = cudaMalloc(&at, b);
+    if (e == cudaErrorMemoryAllocation && b > need) {
+        cudaGetLastError();
+        b = need;
+        e = cudaMalloc(&at, b);
+    }
+    if (e != cudaSuccess) at = nullptr;
+    CUDA_OK(e);
     have = b;
     return at;
 }
